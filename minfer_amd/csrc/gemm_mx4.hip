@@ -1,0 +1,559 @@
+// Products with matrices in microscaled 4-bit numbers (`mx4.h`): out[m][n] (+)= sum_k X'[m][k] W'[n][k] (+ bias[n]), X' the rows x in E2M3.
+//
+//  * `few_kernel`: at most 16 rows as they come (quantised in registers on the way), or up to 64 in E2M3 already: the stream of W bounds it.
+//  * `tile_kernel`: more rows, in E2M3 (`rows_kernel` in front): tiles of the result, operands through LDS, optionally with K cut over blocks.
+//  * `parts_kernel` adds what those blocks left.
+#include <algorithm>
+#include <type_traits>
+
+#include "mx4.h"
+
+enum { EPI_F32 = 0, EPI_ACC_F32 = 1, EPI_BF16 = 2, EPI_SWIGLU = 3 };
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// one value of a result that is not gated
+__device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float v, int epi) {
+  if (epi == EPI_BF16) ((bf16*)C)[at] = (bf16)v;
+  else if (epi == EPI_ACC_F32) ((float*)C)[at] += v;
+  else ((float*)C)[at] = v;
+}
+
+// ------------------------------------------------------------------ rows in E2M3
+// A lane takes a block: a wave four rows and 512 k.  Bound by memory: 2 or 4 bytes a value read, 25/32 written.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned* __restrict__ powers,
+                                                   int m, int m32, int k, int steps, int groups) {
+  const int lane = threadIdx.x & 63, i = lane >> 4, c = lane & 15;
+  const size_t unit = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int four = (int)(unit / groups), group = (int)(unit - (size_t)four * groups);
+  const int row = four * 4 + i;
+  if (four * 4 >= m32 * 32) return;
+  unsigned words[sizeof(T) * 8];
+  mx_load_block<VEC>(x + (size_t)min(row, m - 1) * k, group * 512 + c * 32, row < m ? k : 0, words);
+  unsigned power;
+  const uintx6 six = mx6_block(words, power);
+  const int step = group * 4 + (c >> 2), g = c & 3, r = row & 31;
+  if (step < steps) {
+    unsigned char* tile = codes + ((size_t)(row >> 5) * steps + step) * 3072;
+    *reinterpret_cast<uint4*>(tile + g * 512 + r * 16) = uint4{six[0], six[1], six[2], six[3]};
+    *reinterpret_cast<uint2*>(tile + 2048 + g * 256 + r * 8) = uint2{six[4], six[5]};
+  }
+  unsigned four_powers = power << (8 * (c >> 2));
+  four_powers |= __shfl_xor(four_powers, 4, MF_WAVE);
+  four_powers |= __shfl_xor(four_powers, 8, MF_WAVE);
+  if (c < 4) powers[((size_t)(row >> 5) * groups + group) * 128 + g * 32 + r] = four_powers;
+}
+
+// ------------------------------------------------------------------ few rows
+// A workgroup owns R tiles of 16 matrix rows over the whole of K; its NW waves take the tiles' steps of 128 k in turn, so that at any time they
+// read neighbouring kilobytes, D steps of a wave in flight.  A step of a wave feeds the 16x16x128 instruction: A = 16 matrix rows as they are
+// stored, B = 16 rows of x, whose lane holds one block of one row: quantising it takes no other lane.  The waves' sums meet in LDS and are
+// added in the waves' order.  What bounds it is the stream of the matrix; the rows come from L2 again for every workgroup.
+struct Rows6 { const unsigned char* codes; const unsigned* powers; };
+
+template <typename XT, bool VEC, int MT, int R, int NW, int D, bool PAIR>
+__global__ __launch_bounds__(NW * 64) void few_kernel(const XT* __restrict__ x, Rows6 six, const uint4* __restrict__ codes,
+                                                      const unsigned* __restrict__ powers, const float* __restrict__ bias,
+                                                      void* __restrict__ C, int M, int N, int K, int tiles, int steps, int groups, int epi) {
+  constexpr bool RAW = !std::is_same<XT, void>::value;            // x as it comes, or in E2M3
+  constexpr int W = RAW ? (std::is_same<XT, float>::value ? 32 : 16) : 1;
+  static_assert(!RAW || MT == 1, "rows as they come: at most 16");
+  static_assert(!PAIR || R % 2 == 0, "gate and up tiles in pairs");
+  constexpr int COLS = 16 * R, RS = COLS + 4;
+  __shared__ __attribute__((aligned(16))) float red[NW][16][RS];
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile0 = blockIdx.x * R;
+  const uint4* wtile[R];
+  const unsigned* wpow[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int tile = min(tile0 + j, tiles - 1);
+    wtile[j] = codes + (size_t)tile * steps * 64 + lane;
+    wpow[j] = powers + (size_t)tile * groups * 64 + lane;
+  }
+  floatx4 acc[MT][R];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  uint4 w[D][R];
+  unsigned p[D][R], words[D][W], xp[D][MT];
+  uint4 x4[D][MT];
+  uint2 x2[D][MT];
+  auto load = [&](int s, int t) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      w[s][j] = wtile[j][(size_t)t * 64];
+      p[s][j] = wpow[j][(size_t)(t >> 2) * 64];
+    }
+    if constexpr (RAW) {
+      mx_load_block<VEC>(x + (size_t)min(r16, M - 1) * K, t * 128 + g * 32, r16 < M ? K : 0, words[s]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const unsigned char* tile = six.codes + ((size_t)(i >> 1) * steps + t) * 3072;
+        const int r = (i & 1) * 16 + r16;
+        x4[s][i] = *reinterpret_cast<const uint4*>(tile + g * 512 + r * 16);
+        x2[s][i] = *reinterpret_cast<const uint2*>(tile + 2048 + g * 256 + r * 8);
+        xp[s][i] = six.powers[((size_t)(i >> 1) * groups + (t >> 2)) * 128 + g * 32 + r];
+      }
+    }
+  };
+  auto multiply = [&](int s, int t) {
+    const int by = 8 * (t & 3);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      intx8 b;
+      unsigned power;
+      if constexpr (RAW) {
+        b = mx6_operand(mx6_block(words[s], power));
+      } else {
+        b = intx8{(int)x4[s][i].x, (int)x4[s][i].y, (int)x4[s][i].z, (int)x4[s][i].w, (int)x2[s][i].x, (int)x2[s][i].y, 0, 0};
+        power = xp[s][i] >> by;
+      }
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(w[s][j]), b, acc[i][j], MX_FP4, MX_FP6, 0, (int)(p[s][j] >> by),
+                                                                     0, (int)power);
+    }
+  };
+  const int mine = (steps - wid + NW - 1) / NW;                    // steps of this wave: wid, wid + NW, ... (none: 0)
+#pragma unroll
+  for (int s = 0; s < D; ++s)
+    if (s < mine) load(s, wid + s * NW);
+  for (int base = 0; base < mine; base += D) {
+#pragma unroll
+    for (int s = 0; s < D; ++s)
+      if (base + s < mine) {
+        multiply(s, wid + (base + s) * NW);
+        if (base + s + D < mine) load(s, wid + (base + s + D) * NW);
+      }
+  }
+  // D[n][m]: m = lane % 16, n = 4 (lane / 16) + r
+  for (int i = 0; i < MT; ++i) {
+    if (i) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      floatx4 v = acc[0][j];
+#pragma unroll
+      for (int q = 1; q < MT; ++q)
+        if (i == q) v = acc[q][j];
+      *reinterpret_cast<floatx4*>(&red[wid][r16][j * 16 + 4 * g]) = v;
+    }
+    __syncthreads();
+    constexpr int OUT = PAIR ? COLS / 2 : COLS;
+    for (int e = threadIdx.x; e < 16 * OUT; e += NW * 64) {
+      const int m = i * 16 + e / OUT, c = e % OUT;
+      if (m >= M) break;
+      if constexpr (PAIR) {
+        const int f = tile0 * 8 + c, at = (c >> 4) * 32 + (c & 15);
+        float gate = 0.f, up = 0.f;
+#pragma unroll
+        for (int q = 0; q < NW; ++q) {
+          gate += red[q][e / OUT][at];
+          up += red[q][e / OUT][at + 16];
+        }
+        if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)silu_mul(gate, up);
+      } else {
+        const int n = tile0 * 16 + c;
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < NW; ++q) v += red[q][e / OUT][c];
+        if (n < N) store_one(C, (size_t)m * N + n, bias ? v + bias[n] : v, epi);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ tiles
+// 1 KB from memory to LDS, lane after lane (its first byte in M0); the compiler does not know that it writes there, nor waits for it
+__device__ __forceinline__ void copy_kb(const void* base, unsigned off, unsigned lds_byte) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_byte) : "m0");
+}
+// at most N of this wave's youngest copies are in flight, and all its LDS reads are back; then all waves meet
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+  static_assert(N >= 0 && N < 64, "vmcnt has six bits");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Block number -> (tile row, tile column).  Workgroups go to the 8 XCDs in turn: each gets a contiguous eighth of the tiles, numbered in bands
+// of 8 tile rows, down a band's rows first, so that what an XCD has in flight shares operands in its L2.
+__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int& bm, int& bn) {
+  const int n = tiles_m * tiles_n, per = n / 8, rem = n % 8, x = blockIdx.x % 8;
+  const int at = x * per + min(x, rem) + blockIdx.x / 8;
+  const int band = at / (8 * tiles_n), first = band * 8, rows = min(tiles_m - first, 8), in_band = at - band * 8 * tiles_n;
+  bn = in_band / rows;
+  bm = first + in_band - bn * rows;
+}
+
+template <int BM, int BN>
+struct Tile {
+  static constexpr int I = BM / 64, J = BN / 64;                  // blocks of 32 x 32 results of a wave (2 x 2 waves)
+  static constexpr int STAGES = 3, A_ST = BM / 32 * 3072, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
+  static constexpr int PA = BM / 32 * 512, PW = BN / 16 * 256, POW = PA + PW;                  // powers of 512 k
+  static constexpr int LA = BM / 32 * 3 / 4, LW = BN / 16 / 4, L = LA + LW;                    // copies of a wave and step
+  static constexpr int NPA = BM / 64, NPW = BN / 64, LP = (NPA + NPW + 3) / 4;                 // copies of powers
+  static constexpr int LDS = STAGES * STAGE + 2 * POW;
+  static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+// A workgroup of four waves (one a SIMD) takes a BM x BN tile of results, a wave a quarter of it in blocks of 32 x 32 (instruction 32x32x64).
+// A step is 128 k: its codes are copied into one of three stages as they are stored (that is the order in which the operands' lanes read them,
+// 256 bytes to 16 lanes: no two lanes of a read meet in a bank), two steps ahead; the powers of four steps likewise into one of two places.  A step
+// runs in two halves of 64 k: while the products of one half run, the other half's operands are read; the meeting in the second half
+// says that the next step has landed and that nobody reads the stage before it any more.  Reads and copies are set between the
+// products one by one.
+template <int BM, int BN, bool PAIR>
+__global__ __launch_bounds__(256, 1) void tile_kernel(const unsigned char* __restrict__ a_codes, const unsigned char* __restrict__ a_powers,
+                                                      const unsigned char* __restrict__ w_codes, const unsigned char* __restrict__ w_powers,
+                                                      const float* __restrict__ bias, void* __restrict__ C, float* __restrict__ part, int M,
+                                                      int N, int m32, int w16, int steps, int groups, int tiles_m, int tiles_n,
+                                                      int groups_per_part, int epi) {
+  using TT = Tile<BM, BN>;
+  constexpr int I = TT::I, J = TT::J;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  int bm, bn;
+  tile_of_block(tiles_m, tiles_n, bm, bn);
+  const int g0 = blockIdx.y * groups_per_part, g1 = min(g0 + groups_per_part, groups);
+  const int t0 = g0 * 4, t1 = min(g1 * 4, steps), last = t1 - 1;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wid >> 1, wn = wid & 1;
+  const unsigned lds0 = (unsigned)(uintptr_t)smem;
+
+  // copies: piece q of this wave is piece 4 q + wid of the step
+  const unsigned char *ga[TT::LA], *gw[TT::LW], *gp[TT::LP];
+  unsigned la[TT::LA], lw[TT::LW], lp[TT::LP], off_p[TT::LP];
+  const unsigned off = lane * 16;
+#pragma unroll
+  for (int q = 0; q < TT::LA; ++q) {
+    const int piece = q * 4 + wid, b = piece / 3, at = piece - b * 3;
+    ga[q] = a_codes + (size_t)min(bm * (BM / 32) + b, m32 - 1) * steps * 3072 + at * 1024;
+    la[q] = lds0 + piece * 1024;
+  }
+#pragma unroll
+  for (int q = 0; q < TT::LW; ++q) {
+    const int piece = q * 4 + wid;
+    gw[q] = w_codes + (size_t)min(bn * (BN / 16) + piece, w16 - 1) * steps * 1024;
+    lw[q] = lds0 + TT::A_ST + piece * 1024;
+  }
+#pragma unroll
+  for (int q = 0; q < TT::LP; ++q) {                               // (a piece that two waves copy: the same bytes to the same place)
+    const int piece = min(q * 4 + wid, TT::NPA + TT::NPW - 1);
+    if (piece < TT::NPA) {
+      const int b0 = min(bm * (BM / 32) + piece * 2, m32 - 1), b = min(bm * (BM / 32) + piece * 2 + half, m32 - 1);
+      gp[q] = a_powers + (size_t)b0 * groups * 512;
+      off_p[q] = (unsigned)(b - b0) * groups * 512 + l32 * 16;
+    } else {
+      const int pw = piece - TT::NPA, b0 = min(bn * (BN / 16) + pw * 4, w16 - 1), b = min(bn * (BN / 16) + pw * 4 + (lane >> 4), w16 - 1);
+      gp[q] = w_powers + (size_t)b0 * groups * 256;
+      off_p[q] = (unsigned)(b - b0) * groups * 256 + (lane & 15) * 16;
+    }
+    lp[q] = lds0 + TT::STAGES * TT::STAGE + piece * 1024;
+  }
+  auto copy = [&](int q, int t, int st) {                          // q: 0 .. L - 1
+    const int tc = min(t, last);
+    if (q < TT::LA) copy_kb(ga[q] + (size_t)tc * 3072, off, __builtin_amdgcn_readfirstlane(la[q] + st * TT::STAGE));
+    else copy_kb(gw[q - TT::LA] + (size_t)tc * 1024, off, __builtin_amdgcn_readfirstlane(lw[q - TT::LA] + st * TT::STAGE));
+  };
+  auto copy_powers = [&](int q, int group) {
+    const int gc = min(group, g1 - 1);
+    const bool a = q * 4 + wid < TT::NPA;
+    copy_kb(gp[q] + (size_t)gc * (a ? 512 : 256), off_p[q], __builtin_amdgcn_readfirstlane(lp[q] + (group & 1) * TT::POW));
+  };
+
+  // where this lane's operands lie in a stage
+  const unsigned a16 = wm * I * 3072 + half * 512 + l32 * 16, a8 = wm * I * 3072 + 2048 + half * 256 + l32 * 8;
+  const unsigned hi = l32 >> 4, r16 = lane & 15;
+  const unsigned wb = TT::A_ST + wn * J * 2048 + hi * (PAIR ? 2048 : 1024) + half * 256 + r16 * 16;
+  const unsigned pa = TT::STAGES * TT::STAGE + wm * I * 512 + half * 128 + l32 * 4;
+  const unsigned pw = TT::STAGES * TT::STAGE + TT::PA + wn * J * 512 + hi * (PAIR ? 512 : 256) + half * 64 + r16 * 4;
+  auto w_tile = [](int j) { return PAIR ? (j >> 1) * 4 + (j & 1) : 2 * j; };
+
+  floatx16 acc[I][J];
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  intx8 fa[2][I], fw[2][J];
+  int sa[2][I], sw[2][J];
+  // read i of a half's operands: rows i, then matrix rows i - I, and their powers where a group of four steps begins
+  auto read = [&](int i, auto H, int st, bool begins, int group) {
+    constexpr int h = decltype(H)::value;
+    if (i < I) {
+      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + i * 3072 + h * 1024);
+      const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + i * 3072 + h * 512);
+      fa[h][i] = intx8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, 0, 0};
+      if (begins) sa[h][i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + i * 512 + h * 256);
+    } else {
+      const int j = i - I;
+      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + wb + w_tile(j) * 1024 + h * 512);
+      fw[h][j] = mx4_operand(x);
+      if (begins) sw[h][j] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pw + w_tile(j) * 256 + h * 128);
+    }
+  };
+  using H0 = std::integral_constant<int, 0>;
+  using H1 = std::integral_constant<int, 1>;
+
+#pragma unroll
+  for (int q = 0; q < TT::LP; ++q) copy_powers(q, g0);
+#pragma unroll
+  for (int q = 0; q < TT::L; ++q) copy(q, t0, 0);
+#pragma unroll
+  for (int q = 0; q < TT::L; ++q) copy(q, t0 + 1, 1);
+  wait_and_meet<TT::L>();
+#pragma unroll
+  for (int i = 0; i < I + J; ++i) read(i, H0{}, 0, true, g0);
+
+  int st = 0;
+  auto step = [&](int t, int group, auto S) {
+    constexpr int s = decltype(S)::value;
+    constexpr int NM = I * J, READS = I + J;
+    const int ahead = st == 0 ? 2 : st - 1, next = st == 2 ? 0 : st + 1;
+    // the first half's products; the second half's operands; copies of the step after next
+    constexpr int COPIES = TT::L + (s == 0 ? TT::LP : 0);
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+      const int i = q / J, j = q % J;
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[0][i], fw[0][j], acc[i][j], MX_FP6, MX_FP4, s, sa[0][i], s, sw[0][j]);
+#pragma unroll
+      for (int z = q * READS / NM; z < (q + 1) * READS / NM; ++z) read(z, H1{}, st, s == 0, group);
+#pragma unroll
+      for (int z = q * COPIES / NM; z < (q + 1) * COPIES / NM; ++z) {
+        if (z < TT::L) copy(z, t + 2, ahead);
+        else copy_powers(z - TT::L, group + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (powers of the next group: issued behind the copies of a group's first step, so both its first two steps count them)
+    constexpr int FLIGHT = TT::L + (s < 2 ? TT::LP : 0), BEFORE = NM / 4;
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+      const int i = q / J, j = q % J;
+      if (q == BEFORE) wait_and_meet<FLIGHT>();
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[1][i], fw[1][j], acc[i][j], MX_FP6, MX_FP4, s, sa[1][i], s, sw[1][j]);
+      if (q >= BEFORE) {
+        const int z0 = (q - BEFORE) * READS / (NM - BEFORE), z1 = (q - BEFORE + 1) * READS / (NM - BEFORE);
+#pragma unroll
+        for (int z = z0; z < z1; ++z) read(z, H0{}, next, s == 3, group + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    st = next;
+  };
+  for (int group = g0; group < g1; ++group) {
+    const int t = group * 4;
+    step(t, group, std::integral_constant<int, 0>{});
+    if (t + 1 < t1) step(t + 1, group, std::integral_constant<int, 1>{});
+    if (t + 2 < t1) step(t + 2, group, std::integral_constant<int, 2>{});
+    if (t + 3 < t1) step(t + 3, group, std::integral_constant<int, 3>{});
+  }
+  // (copies past the last step write LDS that nobody reads, but must not outlive the workgroup)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // D[m][n]: n = lane % 32, m = 8 (r / 4) + 4 (lane / 32) + r % 4
+  const int m0 = bm * BM + wm * I * 32 + 4 * half;
+  if (part) {
+    const int width = w16 * 16;
+    part += (size_t)blockIdx.y * M * width;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int n = bn * BN + wn * J * 32 + (w_tile(j) + (PAIR ? 2 : 1) * (int)hi) * 16 + (int)r16;
+      if (n >= width) continue;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = m0 + i * 32 + 8 * (r >> 2) + (r & 3);
+          if (m < M) part[(size_t)m * width + n] = acc[i][j][r];
+        }
+    }
+  } else if constexpr (PAIR) {
+#pragma unroll
+    for (int j = 0; j < J; j += 2) {
+      const int f = (bn * BN + wn * J * 32 + j * 32) / 2 + l32;
+      if (f >= N) continue;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = m0 + i * 32 + 8 * (r >> 2) + (r & 3);
+          if (m < M) ((bf16*)C)[(size_t)m * N + f] = (bf16)silu_mul(acc[i][j][r], acc[i][j + 1][r]);
+        }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int n = bn * BN + wn * J * 32 + j * 32 + l32;
+      if (n >= N) continue;
+      const float b = bias ? bias[n] : 0.f;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = m0 + i * 32 + 8 * (r >> 2) + (r & 3);
+          if (m < M) store_one(C, (size_t)m * N + n, acc[i][j][r] + b, epi);
+        }
+    }
+  }
+}
+
+// The parts of a product whose K was cut, added in their order.  A thread takes four neighbouring matrix rows of one row.
+__global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ part, const float* __restrict__ bias, void* __restrict__ C, int M,
+                                                    int N, int width, int splits, int epi) {
+  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, stride = (size_t)M * width;
+  const int per = (epi == EPI_SWIGLU ? width / 2 : width) / 4;
+  const int m = (int)(at / per), c = (int)(at - (size_t)m * per) * 4;
+  if (m >= M) return;
+  auto sum = [&](int n) {
+    const float4* p = reinterpret_cast<const float4*>(part + (size_t)m * width + n);
+    float4 v = *p;
+    for (int s = 1; s < splits; ++s) {
+      const float4 o = *reinterpret_cast<const float4*>(part + s * stride + (size_t)m * width + n);
+      v.x += o.x;
+      v.y += o.y;
+      v.z += o.z;
+      v.w += o.w;
+    }
+    return v;
+  };
+  if (epi == EPI_SWIGLU) {
+    const float4 g = sum((c >> 4) * 32 + (c & 15)), u = sum((c >> 4) * 32 + 16 + (c & 15));
+    const float y[4] = {silu_mul(g.x, u.x), silu_mul(g.y, u.y), silu_mul(g.z, u.z), silu_mul(g.w, u.w)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < N) ((bf16*)C)[(size_t)m * N + c + i] = (bf16)y[i];
+  } else {
+    const float4 v = sum(c);
+    const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < N) store_one(C, (size_t)m * N + c + i, bias ? y[i] + bias[c + i] : y[i], epi);
+  }
+}
+
+// ------------------------------------------------------------------ which kernel
+// form: 0 `few_kernel` on rows as they come, 1 on rows in E2M3, 2 .. `tile_kernel` of TILE_FORMS[form - 2]; parts of K, groups of 512 k in each
+enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 2 };
+struct Plan { int form, splits, groups; };
+
+static Plan make_plan(int M, int w16, int groups, int n_cu) {
+  if (M <= 16) return Plan{FEW_RAW, 1, groups};
+  if (M <= 64) return Plan{FEW_SIX, 1, groups};
+  constexpr int side[N_TILE_FORMS] = {256, 128};
+  Plan best{TILES, 1, groups};
+  double least = 1e30;
+  for (int f = 0; f < N_TILE_FORMS; ++f) {
+    const long tiles = (long)((M + side[f] - 1) / side[f]) * ((w16 * 16 + side[f] - 1) / side[f]);
+    for (int s = 1; s <= std::min(groups, 16); ++s) {
+      const int per = (groups + s - 1) / s, splits = (groups + per - 1) / per;
+      if (splits != s) continue;
+      const double rounds = (double)((tiles * splits + n_cu - 1) / n_cu);
+      const double work = side[f] == 256 ? 4.0 : 1.2;
+      const double cost = rounds * (per * work + 3.0) + (splits > 1 ? 8.0 + (double)M * w16 * splits / 1e5 : 0.0);
+      if (cost < least) {
+        least = cost;
+        best = Plan{TILES + f, splits, per};
+      }
+    }
+  }
+  return best;
+}
+
+// out: form, parts of K, bytes of scratch for the rows in E2M3, floats of scratch for the parts (64 bits each)
+MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int n_cu, long long* out) {
+  if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
+  const long long w16 = (swiglu ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
+  if (w16 * 16 > (1LL << 30)) return (int)hipErrorInvalidValue;
+  const Plan p = make_plan(M, (int)w16, (int)groups, n_cu);
+  out[0] = p.form;
+  out[1] = p.splits;
+  out[2] = p.form == FEW_RAW ? 0 : m32 * (steps * 3072 + groups * 512);
+  out[3] = p.splits > 1 ? (long long)p.splits * M * w16 * 16 : 0;
+  return 0;
+}
+
+template <int BM, int BN, bool PAIR>
+static int launch_tiles(const unsigned char* six, const void* codes, const void* powers, const float* bias, void* C, float* part, int M, int N,
+                        int m32, int w16, int steps, int groups, const Plan& p, int epi, hipStream_t stream) {
+  using TT = Tile<BM, BN>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<BM, BN, PAIR>), hipFuncAttributeMaxDynamicSharedMemorySize, TT::LDS);
+  if (e != hipSuccess) return (int)e;
+  const int tiles_m = (M + BM - 1) / BM, tiles_n = (w16 * 16 + BN - 1) / BN;
+  tile_kernel<BM, BN, PAIR><<<dim3(tiles_m * tiles_n, p.splits), 256, TT::LDS, stream>>>(
+      six, six + (size_t)m32 * steps * 3072, (const unsigned char*)codes, (const unsigned char*)powers, bias, C, p.splits > 1 ? part : nullptr, M, N,
+      m32, w16, steps, groups, tiles_m, tiles_n, p.groups, epi);
+  return mf_launch_status();
+}
+
+template <typename XT, bool VEC, int MT, int D>
+static int launch_few(const XT* x, const Rows6& six, const void* codes, const void* powers, const float* bias, void* C, int M, int N, int K, int w16,
+                      int steps, int groups, int epi, hipStream_t stream) {
+  if (epi == EPI_SWIGLU)
+    few_kernel<XT, VEC, MT, 2, 8, D, true><<<(w16 + 1) / 2, 512, 0, stream>>>(x, six, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K,
+                                                                            w16, steps, groups, epi);
+  else
+    few_kernel<XT, VEC, MT, 1, 8, D, false><<<w16, 512, 0, stream>>>(x, six, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K, w16,
+                                                                     steps, groups, epi);
+  return mf_launch_status();
+}
+
+// C [M][N] (float32, added to where epi is EPI_ACC_F32, or bfloat16) from x [M][K] (bfloat16 or float32) and the stored [N][K]; EPI_SWIGLU: C is
+// [M][N] bfloat16 and the matrix holds N gate rows and N up rows, tile by tile in turn.  scratch: as `mf_mx4_plan` says, 16-byte aligned.
+MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const void* powers, const float* bias, void* C, void* scratch, float* part,
+                         int M, int N, int K, int epi, int n_cu, hipStream_t stream) {
+  long long sizes[4];
+  const int bad = mf_mx4_plan(M, N, K, epi == EPI_SWIGLU, n_cu, sizes);
+  if (bad) return bad;
+  const int w16 = (epi == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
+  const Plan p = make_plan(M, w16, groups, n_cu);
+  const bool vec = (uintptr_t)x % 16 == 0 && K % (is_bf16 ? 8 : 4) == 0;
+  Rows6 six{(const unsigned char*)scratch, (const unsigned*)((const unsigned char*)scratch + (size_t)m32 * steps * 3072)};
+  if (p.form == FEW_RAW) {
+    auto run = [&](auto T0, auto VEC) {
+      using T = decltype(T0);
+      return launch_few<T, decltype(VEC)::value, 1, sizeof(T) == 2 ? 4 : 2>((const T*)x, six, codes, powers, bias, C, M, N, K, w16, steps, groups,
+                                                                          epi, stream);
+    };
+    if (is_bf16) return vec ? run(bf16{}, std::true_type{}) : run(bf16{}, std::false_type{});
+    return vec ? run(float{}, std::true_type{}) : run(float{}, std::false_type{});
+  }
+  if (!scratch || (p.splits > 1 && !part)) return (int)hipErrorInvalidValue;
+  auto quantise = [&](auto T0, auto VEC) {
+    using T = decltype(T0);
+    const size_t units = (size_t)m32 * 8 * groups;
+    rows_kernel<T, decltype(VEC)::value><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>((const T*)x, (unsigned char*)scratch, (unsigned*)six.powers, M,
+                                                                                        m32, K, steps, groups);
+  };
+  if (is_bf16) vec ? quantise(bf16{}, std::true_type{}) : quantise(bf16{}, std::false_type{});
+  else vec ? quantise(float{}, std::true_type{}) : quantise(float{}, std::false_type{});
+  int rc = mf_launch_status();
+  if (rc) return rc;
+  if (p.form == FEW_SIX) {
+    auto run = [&](auto MT) {
+      return launch_few<void, true, decltype(MT)::value, 4>((const void*)nullptr, six, codes, powers, bias, C, M, N, K, w16, steps, groups, epi, stream);
+    };
+    if (M <= 32) return run(std::integral_constant<int, 2>{});
+    return run(std::integral_constant<int, 4>{});
+  }
+  auto tiles = [&](auto B, auto PAIR) {
+    return launch_tiles<decltype(B)::value, decltype(B)::value, decltype(PAIR)::value>((const unsigned char*)scratch, codes, powers, bias, C, part, M, N,
+                                                                                     m32, w16, steps, groups, p, epi, stream);
+  };
+  using B256 = std::integral_constant<int, 256>;
+  using B128 = std::integral_constant<int, 128>;
+  if (p.form == TILES) rc = epi == EPI_SWIGLU ? tiles(B256{}, std::true_type{}) : tiles(B256{}, std::false_type{});
+  else rc = epi == EPI_SWIGLU ? tiles(B128{}, std::true_type{}) : tiles(B128{}, std::false_type{});
+  if (rc || p.splits == 1) return rc;
+  const size_t per = (size_t)(epi == EPI_SWIGLU ? w16 * 8 : w16 * 16) / 4;
+  parts_kernel<<<(unsigned)((per * M + 255) / 256), 256, 0, stream>>>(part, bias, C, M, N, w16 * 16, p.splits, epi);
+  return mf_launch_status();
+}

@@ -157,6 +157,14 @@ _PROTOTYPES = {
         "mf_gemm_bf16_tile_plan": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P],
         "mf_gemm_bf16_whole_parts": [c_int, c_int, c_int, c_int],
     },
+    "mx4": {
+        "mf_mx4_quantise": [_P, c_int, _P, _P, c_int, c_int, _P],
+        "mf_mx4_dequantise": [_P, _P, _P, c_int, c_int, c_int, _P],
+    },
+    "gemm_mx4": {
+        "mf_mx4_plan": [c_int, c_int, c_int, c_int, c_int, _P],
+        "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P],
+    },
     "attn_tokens_f32": {
         "mf_attn_tokens_f32": [_P, _P, _P, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
                                c_float, c_int, c_int, c_int, _P],
@@ -214,8 +222,8 @@ def _fn(lib: str, name: str, variant: Optional[str] = None):
     if f is None:
         address = ctypes.cast(getattr(build.load(variant or lib), name), c_void_p).value
         kinds = "".join(_KINDS[t] for t in _PROTOTYPES[lib][name])
-        # (what launches ends with the stream; the tile plan ends with the place for its answer)
-        f = (_launch or _native_calls())(address, kinds, kinds.endswith("p") and name != "mf_gemm_bf16_tile_plan")
+        # (what launches ends with the stream; the plans end with the place for their answer)
+        f = (_launch or _native_calls())(address, kinds, kinds.endswith("p") and name not in ("mf_gemm_bf16_tile_plan", "mf_mx4_plan"))
         _functions[key] = f
     return f
 
@@ -2139,6 +2147,127 @@ def linear_gated(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, limit
     _check(_fn("gemm_bf16", "mf_gemm_bf16_gated")(x, k, weight, k, out, m, f, k, int(act), float(limit), gate_logits,
                                                    0 if gate_logits is None else gate_logits.shape[1], _stream()),
            f"gemm_bf16_gated {m}x{f}x{k}")
+
+
+# ------------------------------------------------------------------ matrices in microscaled 4-bit numbers
+def mx4_shapes(rows: int, k: int) -> Tuple[Tuple[int, ...], Tuple[int, ...]]:
+    """Shapes (both uint8) of the codes and of the powers of two that hold a matrix `[rows][k]` in microscaled 4-bit numbers
+    (E2M1; 32 neighbouring values of a row share a power of two), 17/32 of a byte a value.  Codes `[ceil(rows / 16)][ceil(k / 128)][64][16]`:
+    place 16 g + r of a tile holds row r's values 32 g .. 32 g + 31 of the tile's 128, two to a byte, the lower one in the low half.  Powers
+    `[ceil(rows / 16)][ceil(k / 512)][64][4]`: place 16 g + r, byte s: that of row r's block 4 s + g of these 512 values, its exponent + 127
+    (255: the block is NaN).  Past the rows and past k: zeros."""
+    tiles = (rows + 15) // 16
+    return (tiles, (k + 127) // 128, 64, 16), (tiles, (k + 511) // 512, 64, 4)
+
+
+def _mx4_sizes(what: str, *sizes: int) -> None:
+    if min(sizes) < 1 or max(sizes) > 1 << 30:
+        raise KernelError(f"{what}: sizes {sizes} (1 to 2^30)")
+
+
+def mx4_quantise(weight: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor) -> None:
+    """`weight` `[rows][k]` (float32 or bfloat16) into `codes`, `powers` (uint8, see `mx4_shapes`).  A block's power of two is the smallest
+    with which its largest magnitude is at most 7 (which becomes 6: half a step); a value becomes the nearest of 0 0.5 1 1.5 2 3 4 6 times
+    that power, ties to the even code.  A block with an infinity or a NaN is NaN."""
+    _need(weight, "mx4_quantise.weight", _FLOATS)
+    if weight.dim() != 2:
+        raise KernelError(f"mx4_quantise: weight must be a matrix, got {tuple(weight.shape)}")
+    rows, k = weight.shape
+    _mx4_sizes("mx4_quantise", rows, k)
+    shapes = mx4_shapes(rows, k)
+    _need(codes, "mx4_quantise.codes", torch.uint8, shapes[0])
+    _need(powers, "mx4_quantise.powers", torch.uint8, shapes[1])
+    _aligned("mx4_quantise", codes=codes, powers=powers)
+    _check(_fn("mx4", "mf_mx4_quantise")(weight, _is_bf16(weight), codes, powers, rows, k, _stream()), f"mx4_quantise {rows}x{k}")
+
+
+def mx4_dequantise(codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor) -> None:
+    """The values that `codes`, `powers` hold, into `out` `[rows][k]` (float32 or bfloat16; both hold them exactly)."""
+    _need(out, "mx4_dequantise.out", _FLOATS)
+    if out.dim() != 2:
+        raise KernelError(f"mx4_dequantise: out must be a matrix, got {tuple(out.shape)}")
+    rows, k = out.shape
+    _mx4_sizes("mx4_dequantise", rows, k)
+    shapes = mx4_shapes(rows, k)
+    _need(codes, "mx4_dequantise.codes", torch.uint8, shapes[0])
+    _need(powers, "mx4_dequantise.powers", torch.uint8, shapes[1])
+    _aligned("mx4_dequantise", codes=codes, powers=powers)
+    _check(_fn("mx4", "mf_mx4_dequantise")(codes, powers, out, _is_bf16(out), rows, k, _stream()), f"mx4_dequantise {rows}x{k}")
+
+
+def _aligned(what: str, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.data_ptr() % 16:
+            raise KernelError(f"{what}.{name}: must begin at a multiple of 16 bytes")
+
+
+@functools.lru_cache(maxsize=4096)
+def _mx4_plan(m: int, n: int, k: int, swiglu: bool, n_cu: int) -> Tuple[int, int, int, int]:
+    out = (c_int64 * 4)()
+    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, 1 if swiglu else 0, n_cu, out)
+    if rc != 0:
+        raise KernelError(f"mx4_linear: error {rc} for m {m}, n {n}, k {k}")
+    return tuple(out)
+
+
+def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
+                 epi: int) -> None:
+    m, k = x.shape
+    n = out.shape[1]
+    if m == 0:
+        return
+    _aligned(what, codes=codes, powers=powers)
+    n_cu = cu_count()
+    _, _, six, parts = _mx4_plan(m, n, k, epi == EPI_SWIGLU, n_cu)
+    scratch = torch.empty(six, dtype=torch.uint8, device=x.device) if six else None
+    part = torch.empty(parts, dtype=torch.float32, device=x.device) if parts else None
+    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, n_cu, _stream()),
+           f"{what} {m}x{n}x{k}")
+
+
+def mx4_linear(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
+               accumulate: bool = False) -> None:
+    """out (+)= x' W'^T (+ bias): W' the matrix `[n][k]` that `codes`, `powers` hold in microscaled 4-bit numbers (`mx4_quantise`), x' the rows
+    of `x` `[m][k]` (float32 or bfloat16) in microscaled 6-bit ones (E2M3: blocks of 32, the smallest power of two with which the largest magnitude is
+    at most 7.5, the nearest value, ties to even), which the product makes on its way.  Sums and `bias` are 32-bit; `out` `[m][n]` is float32, or
+    bfloat16 where it is stored.  A row of x with an infinity or a NaN gives NaN."""
+    _need(x, "mx4_linear.x", _FLOATS)
+    _need(out, "mx4_linear.out", _FLOATS)
+    if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0]:
+        raise KernelError(f"mx4_linear: x {tuple(x.shape)}, out {tuple(out.shape)}")
+    k, n = x.shape[1], out.shape[1]
+    _mx4_sizes("mx4_linear", n, k)
+    shapes = mx4_shapes(n, k)
+    _need(codes, "mx4_linear.codes", torch.uint8, shapes[0])
+    _need(powers, "mx4_linear.powers", torch.uint8, shapes[1])
+    if bias is not None:
+        _need(bias, "mx4_linear.bias", torch.float32, (n,))
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("mx4_linear: accumulation needs a float32 output")
+    _mx4_product("mx4_linear", x, codes, powers, bias, out, EPI_BF16 if out.dtype == torch.bfloat16 else EPI_ACC_F32 if accumulate else EPI_F32)
+
+
+def mx4_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """The codes (or the powers) of a gate and an up matrix of the same sizes as `mx4_linear_swiglu` reads them: tile by tile in turn,
+    `[2 ceil(rows / 16)][..]`.  Leading dimensions (experts) stay."""
+    if gate.shape != up.shape or gate.dim() < 4:
+        raise KernelError(f"mx4_pairs: gate {tuple(gate.shape)}, up {tuple(up.shape)}")
+    return torch.stack([gate, up], dim=-4).flatten(-5, -4).contiguous()
+
+
+def mx4_linear_swiglu(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor) -> None:
+    """out = silu(x' G'^T) * (x' U'^T), rounded once to bfloat16, in one product; `codes`, `powers`: `mx4_pairs` of those of G and U `[f][k]`;
+    x' as in `mx4_linear`, `out` bfloat16 `[m][f]`."""
+    _need(x, "mx4_linear_swiglu.x", _FLOATS)
+    _need(out, "mx4_linear_swiglu.out", torch.bfloat16)
+    if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0]:
+        raise KernelError(f"mx4_linear_swiglu: x {tuple(x.shape)}, out {tuple(out.shape)}")
+    k, f = x.shape[1], out.shape[1]
+    _mx4_sizes("mx4_linear_swiglu", 2 * f, k)
+    (tiles, *c), (_, *p) = mx4_shapes(f, k)
+    _need(codes, "mx4_linear_swiglu.codes", torch.uint8, (2 * tiles, *c))
+    _need(powers, "mx4_linear_swiglu.powers", torch.uint8, (2 * tiles, *p))
+    _mx4_product("mx4_linear_swiglu", x, codes, powers, None, out, EPI_SWIGLU)
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
