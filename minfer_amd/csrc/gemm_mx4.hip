@@ -10,7 +10,11 @@
 
 enum { EPI_F32 = 0, EPI_ACC_F32 = 1, EPI_BF16 = 2, EPI_SWIGLU = 3 };
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) u by the hardware's 2^x and reciprocal: off by some |g| 2^-24 of itself, far inside the rounding to bfloat16 behind it (expf and a
+// division take as long as the stores of a prompt's tile: 389 us instead of SILU for 4,096 rows of 37,888 x 3,584)
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
+}
 
 // one value of a result that is not gated
 __device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float v, int epi) {
@@ -192,30 +196,76 @@ __device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int& bm,
   bm = first + in_band - bn * rows;
 }
 
-template <int BM, int BN>
+template <int BM, int BN, int STAGES_>
 struct Tile {
   static constexpr int I = BM / 64, J = BN / 64;                  // blocks of 32 x 32 results of a wave (2 x 2 waves)
-  static constexpr int STAGES = 3, A_ST = BM / 32 * 3072, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
+  static constexpr int STAGES = STAGES_, A_ST = BM / 32 * 3072, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
   static constexpr int PA = BM / 32 * 512, PW = BN / 16 * 256, POW = PA + PW;                  // powers of 512 k
   static constexpr int LA = BM / 32 * 3 / 4, LW = BN / 16 / 4, L = LA + LW;                    // copies of a wave and step
   static constexpr int NPA = BM / 64, NPW = BN / 64, LP = (NPA + NPW + 3) / 4;                 // copies of powers
   static constexpr int LDS = STAGES * STAGE + 2 * POW;
-  static_assert(LDS <= 160 * 1024, "LDS");
+  static constexpr int ROW = (BN / 2 + 4) * 4;                    // bytes of a row of a wave's results on their way out (16 more: no two rows in a bank)
+  static_assert(LDS <= 160 * 1024 && 4 * 32 * ROW <= LDS, "LDS");
 };
+
+// Results of more bytes than the L2s hold are marked: who reads them next finds them in no L2 anyway, and so they do not push the operands out.
+// (4,096 rows, swiglu of 37,888 x 3,584, 155 MB: 355 us, marked 329; 16,384 x 4,096 in 32 bits, 268 MB: 204, 189.)
+__device__ __forceinline__ bool leaves_once(size_t bytes) { return bytes > (32u << 20); }
+
+// `rows` rows of COLS results that lie in LDS, `pitch` bytes to a row, to C [..][N] from row m_first and column n_first on: 32-bit ones (with a
+// bias, or added to C), or bfloat16.  16 bytes a lane where C's rows allow it.  `once`: marked as not read again soon (`leaves_once`).
+template <int COLS, int EPI>
+__device__ __forceinline__ void leave_rows(const unsigned char* __restrict__ own, int pitch, void* __restrict__ C, int m_first, int rows, int n_first,
+                                           int N, const float* __restrict__ bias, bool once, int lane) {
+  using T = typename std::conditional<EPI == EPI_BF16, bf16, float>::type;
+  constexpr int PER = 16 / sizeof(T), LANES = COLS / PER, AT_ONCE = 64 / LANES;      // results and lanes of a store, rows of one
+  const int c = lane % LANES * PER, n = n_first + c, valid = N - n;
+  if (valid <= 0) return;
+  const bool whole = valid >= PER && N % PER == 0 && (uintptr_t)C % 16 == 0;
+  T* to = (T*)C + (size_t)m_first * N + n;
+  float b[PER];
+  if constexpr (EPI != EPI_BF16) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) b[x] = bias && x < valid ? bias[n + x] : 0.f;
+  }
+#pragma unroll 4
+  for (int r = lane / LANES; r < rows; r += AT_ONCE) {
+    alignas(16) T v[PER];
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(own + r * pitch + c * sizeof(T));
+    T* at = to + (size_t)r * N;
+    if constexpr (EPI != EPI_BF16) {
+#pragma unroll
+      for (int x = 0; x < PER; ++x) v[x] += b[x];
+    }
+    if (whole) {
+      if constexpr (EPI == EPI_ACC_F32) {
+        const float4 old = *reinterpret_cast<const float4*>(at);
+        v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
+      }
+      typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+      if (once) __builtin_nontemporal_store(*reinterpret_cast<const uintx4*>(v), reinterpret_cast<uintx4*>(at));
+      else *reinterpret_cast<uintx4*>(at) = *reinterpret_cast<const uintx4*>(v);
+    } else {
+#pragma unroll
+      for (int x = 0; x < PER; ++x)
+        if (x < valid) at[x] = EPI == EPI_ACC_F32 ? (T)((float)at[x] + (float)v[x]) : v[x];
+    }
+  }
+}
 
 // A workgroup of four waves (one a SIMD) takes a BM x BN tile of results, a wave a quarter of it in blocks of 32 x 32 (instruction 32x32x64).
 // A step is 128 k: its codes are copied into one of three stages as they are stored (that is the order in which the operands' lanes read them,
-// 256 bytes to 16 lanes: no two lanes of a read meet in a bank), two steps ahead; the powers of four steps likewise into one of two places.  A step
-// runs in two halves of 64 k: while the products of one half run, the other half's operands are read; the meeting in the second half
-// says that the next step has landed and that nobody reads the stage before it any more.  Reads and copies are set between the
-// products one by one.
-template <int BM, int BN, bool PAIR>
-__global__ __launch_bounds__(256, 1) void tile_kernel(const unsigned char* __restrict__ a_codes, const unsigned char* __restrict__ a_powers,
+// 256 bytes to 16 lanes: no two lanes of a read meet in a bank), up to three steps ahead; the powers of four steps likewise into one of two
+// places.  A step runs in two halves of 64 k: while the products of one half run, the other half's operands are read; the meeting in the second
+// half says that the next step has landed and that nobody reads this one's stage any more.  Reads and copies are set between the products one
+// by one.
+template <int BM, int BN, int STAGES, int PER_CU, bool PAIR>
+__global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* __restrict__ a_codes, const unsigned char* __restrict__ a_powers,
                                                       const unsigned char* __restrict__ w_codes, const unsigned char* __restrict__ w_powers,
                                                       const float* __restrict__ bias, void* __restrict__ C, float* __restrict__ part, int M,
                                                       int N, int m32, int w16, int steps, int groups, int tiles_m, int tiles_n,
                                                       int groups_per_part, int epi) {
-  using TT = Tile<BM, BN>;
+  using TT = Tile<BM, BN, STAGES>;
   constexpr int I = TT::I, J = TT::J;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int bm, bn;
@@ -271,10 +321,9 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(const unsigned char* __res
   // where this lane's operands lie in a stage
   const unsigned a16 = wm * I * 3072 + half * 512 + l32 * 16, a8 = wm * I * 3072 + 2048 + half * 256 + l32 * 8;
   const unsigned hi = l32 >> 4, r16 = lane & 15;
-  const unsigned wb = TT::A_ST + wn * J * 2048 + hi * (PAIR ? 2048 : 1024) + half * 256 + r16 * 16;
+  const unsigned wb = TT::A_ST + wn * J * 2048 + hi * 1024 + half * 256 + r16 * 16;
   const unsigned pa = TT::STAGES * TT::STAGE + wm * I * 512 + half * 128 + l32 * 4;
-  const unsigned pw = TT::STAGES * TT::STAGE + TT::PA + wn * J * 512 + hi * (PAIR ? 512 : 256) + half * 64 + r16 * 4;
-  auto w_tile = [](int j) { return PAIR ? (j >> 1) * 4 + (j & 1) : 2 * j; };
+  const unsigned pw = TT::STAGES * TT::STAGE + TT::PA + wn * J * 512 + hi * 256 + half * 64 + r16 * 4;
 
   floatx16 acc[I][J];
 #pragma unroll
@@ -295,55 +344,59 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(const unsigned char* __res
       if (begins) sa[h][i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + i * 512 + h * 256);
     } else {
       const int j = i - I;
-      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + wb + w_tile(j) * 1024 + h * 512);
+      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + wb + j * 2048 + h * 512);
       fw[h][j] = mx4_operand(x);
-      if (begins) sw[h][j] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pw + w_tile(j) * 256 + h * 128);
+      if (begins) sw[h][j] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pw + j * 512 + h * 128);
     }
   };
   using H0 = std::integral_constant<int, 0>;
   using H1 = std::integral_constant<int, 1>;
+  // products of a half, in front of its meeting and behind it; operand reads of a half; copies of a step that are set out behind the meeting of
+  // the step three before it (the rest: in the first half of the next one)
+  constexpr int NM = I * J, BEFORE = NM / 4, BEHIND = NM - BEFORE, READS = I + J, EARLY = STAGES == 2 ? TT::L : TT::L * BEHIND / (NM + BEHIND);
 
 #pragma unroll
   for (int q = 0; q < TT::LP; ++q) copy_powers(q, g0);
 #pragma unroll
-  for (int q = 0; q < TT::L; ++q) copy(q, t0, 0);
+  for (int t = 0; t < STAGES; ++t)
 #pragma unroll
-  for (int q = 0; q < TT::L; ++q) copy(q, t0 + 1, 1);
-  wait_and_meet<TT::L>();
+    for (int q = 0; q < (t == STAGES - 1 ? EARLY : TT::L); ++q) copy(q, t0 + t, t);
+  wait_and_meet<(STAGES - 2) * TT::L + EARLY>();
 #pragma unroll
   for (int i = 0; i < I + J; ++i) read(i, H0{}, 0, true, g0);
 
   int st = 0;
   auto step = [&](int t, int group, auto S) {
     constexpr int s = decltype(S)::value;
-    constexpr int NM = I * J, READS = I + J;
-    const int ahead = st == 0 ? 2 : st - 1, next = st == 2 ? 0 : st + 1;
-    // the first half's products; the second half's operands; copies of the step after next
-    constexpr int COPIES = TT::L + (s == 0 ? TT::LP : 0);
+    const int next = st == STAGES - 1 ? 0 : st + 1;
+    // the first half's products; the second half's operands, the rest of the copies of the step after next
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
       const int i = q / J, j = q % J;
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[0][i], fw[0][j], acc[i][j], MX_FP6, MX_FP4, s, sa[0][i], s, sw[0][j]);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[0][j], fa[0][i], acc[i][j], MX_FP4, MX_FP6, s, sw[0][j], s, sa[0][i]);
 #pragma unroll
       for (int z = q * READS / NM; z < (q + 1) * READS / NM; ++z) read(z, H1{}, st, s == 0, group);
 #pragma unroll
-      for (int z = q * COPIES / NM; z < (q + 1) * COPIES / NM; ++z) {
-        if (z < TT::L) copy(z, t + 2, ahead);
-        else copy_powers(z - TT::L, group + 1);
-      }
+      for (int z = q * (TT::L - EARLY) / NM; z < (q + 1) * (TT::L - EARLY) / NM; ++z) copy(EARLY + z, t + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // (powers of the next group: issued behind the copies of a group's first step, so both its first two steps count them)
-    constexpr int FLIGHT = TT::L + (s < 2 ? TT::LP : 0), BEFORE = NM / 4;
+    // the second half's; behind the meeting this stage is free for the step after next but one, and the next step's operands are here.
+    // In flight at the meeting: a step's copies, and at a group's second one the powers of the next group (set out behind the first).
+    constexpr int FLIGHT = (STAGES - 2) * TT::L + (s == 1 ? TT::LP : 0), COPIES = EARLY + (s == 0 ? TT::LP : 0);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
       const int i = q / J, j = q % J;
       if (q == BEFORE) wait_and_meet<FLIGHT>();
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[1][i], fw[1][j], acc[i][j], MX_FP6, MX_FP4, s, sa[1][i], s, sw[1][j]);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[1][j], fa[1][i], acc[i][j], MX_FP4, MX_FP6, s, sw[1][j], s, sa[1][i]);
       if (q >= BEFORE) {
-        const int z0 = (q - BEFORE) * READS / (NM - BEFORE), z1 = (q - BEFORE + 1) * READS / (NM - BEFORE);
+        const int b = q - BEFORE;
 #pragma unroll
-        for (int z = z0; z < z1; ++z) read(z, H0{}, next, s == 3, group + 1);
+        for (int z = b * READS / BEHIND; z < (b + 1) * READS / BEHIND; ++z) read(z, H0{}, next, s == 3, group + 1);
+#pragma unroll
+        for (int z = b * COPIES / BEHIND; z < (b + 1) * COPIES / BEHIND; ++z) {
+          if (z < EARLY) copy(z, t + STAGES, st);
+          else copy_powers(z - EARLY, group + 1);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -359,50 +412,61 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(const unsigned char* __res
   // (copies past the last step write LDS that nobody reads, but must not outlive the workgroup)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-  // D[m][n]: n = lane % 32, m = 8 (r / 4) + 4 (lane / 32) + r % 4
-  const int m0 = bm * BM + wm * I * 32 + 4 * half;
-  if (part) {
-    const int width = w16 * 16;
-    part += (size_t)blockIdx.y * M * width;
+  __syncthreads();                                                 // (nobody reads the stages any more)
+  // D[n][m]: m = lane % 32, n = 8 (r / 4) + 4 (lane / 32) + r % 4 (gate rows the first 16, up rows the others): a lane holds four neighbouring
+  // results of a row.  32 rows at a time by way of LDS, so that a store takes 16 bytes a lane and whole lines of a row (straight from the
+  // registers, four bytes a lane: 63 us for 2,048 rows of 4,608 x 3,584 that take 35 so).
+  unsigned char* own = smem + wid * 32 * TT::ROW;
+  const bool once = leaves_once((size_t)M * N * (PAIR || epi == EPI_BF16 ? 2 : 4));
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int n = bn * BN + wn * J * 32 + (w_tile(j) + (PAIR ? 2 : 1) * (int)hi) * 16 + (int)r16;
-      if (n >= width) continue;
+  for (int i = 0; i < I; ++i) {
+    const int m_first = bm * BM + wm * I * 32 + i * 32;
+    if (m_first >= M) continue;
+    const int rows = min(32, M - m_first);
+    auto floats = [&]() {
 #pragma unroll
-      for (int i = 0; i < I; ++i)
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int m = m0 + i * 32 + 8 * (r >> 2) + (r & 3);
-          if (m < M) part[(size_t)m * width + n] = acc[i][j][r];
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<floatx4*>(own + l32 * TT::ROW + (j * 32 + q * 8 + half * 4) * 4) =
+              floatx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    };
+    if (part) {
+      floats();
+      __builtin_amdgcn_wave_barrier();
+      leave_rows<J * 32, EPI_F32>(own, TT::ROW, part + (size_t)blockIdx.y * M * (w16 * 16), m_first, rows, bn * BN + wn * J * 32, w16 * 16, nullptr, false, lane);
+    } else if constexpr (PAIR) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          bf16x4 y;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) y[x] = (bf16)silu_mul(acc[i][j][4 * q + x], acc[i][j][8 + 4 * q + x]);
+          *reinterpret_cast<bf16x4*>(own + l32 * TT::ROW + (j * 16 + q * 8 + half * 4) * 2) = y;
         }
-    }
-  } else if constexpr (PAIR) {
+      __builtin_amdgcn_wave_barrier();
+      leave_rows<J * 16, EPI_BF16>(own, TT::ROW, C, m_first, rows, bn * (BN / 2) + wn * J * 16, N, nullptr, once, lane);
+    } else if (epi == EPI_BF16) {
 #pragma unroll
-    for (int j = 0; j < J; j += 2) {
-      const int f = (bn * BN + wn * J * 32 + j * 32) / 2 + l32;
-      if (f >= N) continue;
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < I; ++i)
+        for (int q = 0; q < 4; ++q) {
+          const int n = bn * BN + wn * J * 32 + j * 32 + q * 8 + half * 4;
+          bf16x4 y;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int m = m0 + i * 32 + 8 * (r >> 2) + (r & 3);
-          if (m < M) ((bf16*)C)[(size_t)m * N + f] = (bf16)silu_mul(acc[i][j][r], acc[i][j + 1][r]);
+          for (int x = 0; x < 4; ++x) y[x] = (bf16)(acc[i][j][4 * q + x] + (bias && n + x < N ? bias[n + x] : 0.f));
+          *reinterpret_cast<bf16x4*>(own + l32 * TT::ROW + (j * 32 + q * 8 + half * 4) * 2) = y;
         }
+      __builtin_amdgcn_wave_barrier();
+      leave_rows<J * 32, EPI_BF16>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 32, N, nullptr, once, lane);
+    } else {
+      floats();
+      __builtin_amdgcn_wave_barrier();
+      if (epi == EPI_ACC_F32) leave_rows<J * 32, EPI_ACC_F32>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 32, N, bias, false, lane);
+      else leave_rows<J * 32, EPI_F32>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 32, N, bias, once, lane);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int n = bn * BN + wn * J * 32 + j * 32 + l32;
-      if (n >= N) continue;
-      const float b = bias ? bias[n] : 0.f;
-#pragma unroll
-      for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int m = m0 + i * 32 + 8 * (r >> 2) + (r & 3);
-          if (m < M) store_one(C, (size_t)m * N + n, acc[i][j][r] + b, epi);
-        }
-    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -442,22 +506,22 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
 
 // ------------------------------------------------------------------ which kernel
 // form: 0 `few_kernel` on rows as they come, 1 on rows in E2M3, 2 .. `tile_kernel` of TILE_FORMS[form - 2]; parts of K, groups of 512 k in each
-enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 2 };
+enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 3 };
 struct Plan { int form, splits, groups; };
 
 static Plan make_plan(int M, int w16, int groups, int n_cu) {
   if (M <= 16) return Plan{FEW_RAW, 1, groups};
   if (M <= 64) return Plan{FEW_SIX, 1, groups};
-  constexpr int side[N_TILE_FORMS] = {256, 128};
+  constexpr int tile_m[N_TILE_FORMS] = {256, 256, 128}, tile_n[N_TILE_FORMS] = {256, 128, 128};
   Plan best{TILES, 1, groups};
   double least = 1e30;
   for (int f = 0; f < N_TILE_FORMS; ++f) {
-    const long tiles = (long)((M + side[f] - 1) / side[f]) * ((w16 * 16 + side[f] - 1) / side[f]);
+    const long tiles = (long)((M + tile_m[f] - 1) / tile_m[f]) * ((w16 * 16 + tile_n[f] - 1) / tile_n[f]);
     for (int s = 1; s <= std::min(groups, 16); ++s) {
       const int per = (groups + s - 1) / s, splits = (groups + per - 1) / per;
       if (splits != s) continue;
       const double rounds = (double)((tiles * splits + n_cu - 1) / n_cu);
-      const double work = side[f] == 256 ? 4.0 : 1.2;
+      const double work = f == 0 ? 4.0 : f == 1 ? 2.2 : 1.2;
       const double cost = rounds * (per * work + 3.0) + (splits > 1 ? 8.0 + (double)M * w16 * splits / 1e5 : 0.0);
       if (cost < least) {
         least = cost;
@@ -481,14 +545,14 @@ MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int n_cu, long long* out
   return 0;
 }
 
-template <int BM, int BN, bool PAIR>
+template <int BM, int BN, int STAGES, int PER_CU, bool PAIR>
 static int launch_tiles(const unsigned char* six, const void* codes, const void* powers, const float* bias, void* C, float* part, int M, int N,
                         int m32, int w16, int steps, int groups, const Plan& p, int epi, hipStream_t stream) {
-  using TT = Tile<BM, BN>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<BM, BN, PAIR>), hipFuncAttributeMaxDynamicSharedMemorySize, TT::LDS);
+  using TT = Tile<BM, BN, STAGES>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<BM, BN, STAGES, PER_CU, PAIR>), hipFuncAttributeMaxDynamicSharedMemorySize, TT::LDS);
   if (e != hipSuccess) return (int)e;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (w16 * 16 + BN - 1) / BN;
-  tile_kernel<BM, BN, PAIR><<<dim3(tiles_m * tiles_n, p.splits), 256, TT::LDS, stream>>>(
+  tile_kernel<BM, BN, STAGES, PER_CU, PAIR><<<dim3(tiles_m * tiles_n, p.splits), 256, TT::LDS, stream>>>(
       six, six + (size_t)m32 * steps * 3072, (const unsigned char*)codes, (const unsigned char*)powers, bias, C, p.splits > 1 ? part : nullptr, M, N,
       m32, w16, steps, groups, tiles_m, tiles_n, p.groups, epi);
   return mf_launch_status();
@@ -544,14 +608,19 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
     if (M <= 32) return run(std::integral_constant<int, 2>{});
     return run(std::integral_constant<int, 4>{});
   }
-  auto tiles = [&](auto B, auto PAIR) {
-    return launch_tiles<decltype(B)::value, decltype(B)::value, decltype(PAIR)::value>((const unsigned char*)scratch, codes, powers, bias, C, part, M, N,
+  auto tiles = [&](auto BM, auto BN, auto STAGES, auto PER_CU, auto PAIR) {
+    return launch_tiles<decltype(BM)::value, decltype(BN)::value, decltype(STAGES)::value, decltype(PER_CU)::value, decltype(PAIR)::value>((const unsigned char*)scratch, codes, powers, bias, C, part, M, N,
                                                                                      m32, w16, steps, groups, p, epi, stream);
   };
-  using B256 = std::integral_constant<int, 256>;
-  using B128 = std::integral_constant<int, 128>;
-  if (p.form == TILES) rc = epi == EPI_SWIGLU ? tiles(B256{}, std::true_type{}) : tiles(B256{}, std::false_type{});
-  else rc = epi == EPI_SWIGLU ? tiles(B128{}, std::true_type{}) : tiles(B128{}, std::false_type{});
+  auto choose = [&](auto PAIR) {
+    using std::integral_constant;
+    switch (p.form) {
+      case TILES: return tiles(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 3>{}, integral_constant<int, 1>{}, PAIR);
+      case TILES + 1: return tiles(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, PAIR);
+      default: return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 3>{}, integral_constant<int, 2>{}, PAIR);
+    }
+  };
+  rc = epi == EPI_SWIGLU ? choose(std::true_type{}) : choose(std::false_type{});
   if (rc || p.splits == 1) return rc;
   const size_t per = (size_t)(epi == EPI_SWIGLU ? w16 * 8 : w16 * 16) / 4;
   parts_kernel<<<(unsigned)((per * M + 255) / 256), 256, 0, stream>>>(part, bias, C, M, N, w16 * 16, p.splits, epi);

@@ -31,6 +31,7 @@ LIBRARIES: Dict[str, str] = {
     "gemm_bf16": "gemm_bf16.hip",
     "mx4": "mx4.hip",
     "gemm_mx4": "gemm_mx4.hip",
+    "moe_mx4": "moe_mx4.hip",
     "attn_tokens_f32": "attn_tokens_f32.hip",
     "attn_prompt_f32": "attn_prompt_f32.hip",
     "attn_decode_bf16": "attn_decode_bf16.hip",
@@ -53,6 +54,7 @@ DEFINES: Dict[str, List[str]] = {}
 HEADERS = {"host_random": ["random_normal.h"],
            "mx4": ["common.h", "mx4.h"],
            "gemm_mx4": ["common.h", "mx4.h"],
+           "moe_mx4": ["common.h", "mx4.h"],
            "host_call": [],
            "elementwise": ["common.h", "random_normal.h"],
            "attn_tokens_f32": ["common.h", "attn_tokens_impl.h"],

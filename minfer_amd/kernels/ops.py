@@ -165,6 +165,10 @@ _PROTOTYPES = {
         "mf_mx4_plan": [c_int, c_int, c_int, c_int, c_int, _P],
         "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P],
     },
+    "moe_mx4": {
+        "mf_mx4_moe": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+                       c_int, _P],
+    },
     "attn_tokens_f32": {
         "mf_attn_tokens_f32": [_P, _P, _P, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
                                c_float, c_int, c_int, c_int, _P],
@@ -1506,6 +1510,48 @@ def moe_sparse(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, chose
     _check(_fn("moe", "mf_moe_sparse")(x, gate_up, down, chosen, weights, y, rows, out,
                                         _is_bf16(x), n_tok, top, n_experts, F, K, N, float(limit), int(act),
                                         1 if accumulate else 0, 1 if hands_on else 0, _stream()), "moe_sparse")
+
+
+def mx4_moe_sparse(x: torch.Tensor, gate_up: torch.Tensor, gate_up_powers: torch.Tensor, down: torch.Tensor, down_powers: torch.Tensor,
+                   chosen: torch.Tensor, weights: torch.Tensor, out: torch.Tensor, ff: int, limit: float = 0.0, act: int = 0,
+                   accumulate: bool = True, hands_on: bool = False) -> None:
+    """`moe_sparse` for experts in microscaled 4-bit numbers, in two kernels: `gate_up`, `gate_up_powers` `[experts][2 tiles]..` (`mx4_pairs` of
+    an expert's gate and up matrices `[ff][K]`), `down`, `down_powers` `[experts]..` (`[N][ff]`, see `mx4_shapes`); x `[tokens][K]`, float32
+    or bfloat16, and the activations (rounded to bfloat16 first) meet the matrices as the rows of `mx4_linear` do.  out `[tokens][N]`, float32
+    (+)= the weighted sum of the chosen experts' outputs, or bfloat16 (stored).  A choice that names no expert adds nothing; with
+    `hands_on` one from `experts` on hands the token's x on."""
+    _need(x, "mx4_moe_sparse.x", _FLOATS)
+    _need(out, "mx4_moe_sparse.out", _FLOATS)
+    if x.dim() != 2 or out.dim() != 2 or chosen.dim() != 2 or gate_up.dim() != 5 or out.shape[0] != x.shape[0]:
+        raise KernelError(f"mx4_moe_sparse: x {tuple(x.shape)}, out {tuple(out.shape)}, chosen {tuple(chosen.shape)}, gate_up {tuple(gate_up.shape)}")
+    n_tok, K = x.shape
+    N, E, top = out.shape[1], gate_up.shape[0], chosen.shape[1]
+    _mx4_sizes("mx4_moe_sparse", K, N, ff)
+    (tiles, *up_codes), (_, *up_powers) = mx4_shapes(ff, K)
+    down_codes, down_power = mx4_shapes(N, ff)
+    _need(gate_up, "mx4_moe_sparse.gate_up", torch.uint8, (E, 2 * tiles, *up_codes))
+    _need(gate_up_powers, "mx4_moe_sparse.gate_up_powers", torch.uint8, (E, 2 * tiles, *up_powers))
+    _need(down, "mx4_moe_sparse.down", torch.uint8, (E, *down_codes))
+    _need(down_powers, "mx4_moe_sparse.down_powers", torch.uint8, (E, *down_power))
+    _need(chosen, "mx4_moe_sparse.chosen", torch.int32, (n_tok, top))
+    _need(weights, "mx4_moe_sparse.weights", torch.float32, (n_tok, top))
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("mx4_moe_sparse: accumulation needs a float32 output")
+    if hands_on and K != N:
+        raise KernelError(f"mx4_moe_sparse: inputs of {K} values cannot stand for outputs of {N}")
+    if act not in MOE_ACTS.values():
+        raise KernelError(f"mx4_moe_sparse: activation {act} (one of {MOE_ACTS})")
+    if n_tok == 0:
+        return
+    if not 1 <= E <= MOE_MAX_EXPERTS or not 1 <= top <= 64 or n_tok > MOE_SPARSE_TOKENS or n_tok * top > MOE_SPARSE_PAIRS:
+        raise KernelError(f"mx4_moe_sparse: {n_tok} tokens with {top} of {E} experts each; it takes {MOE_SPARSE_TOKENS} tokens, "
+                          f"{MOE_SPARSE_PAIRS} pairs and {MOE_MAX_EXPERTS} experts")
+    _aligned("mx4_moe_sparse", gate_up=gate_up, gate_up_powers=gate_up_powers, down=down, down_powers=down_powers)
+    y = torch.empty((n_tok * top, 16 * tiles), dtype=torch.bfloat16, device=x.device)
+    _check(_fn("moe_mx4", "mf_mx4_moe")(x, _is_bf16(x), gate_up, gate_up_powers, down, down_powers, chosen, weights, y, out, _is_bf16(out), n_tok,
+                                        top, E, ff, K, N, float(limit), int(act), 1 if accumulate else 0, 1 if hands_on else 0, _stream()),
+           "mx4_moe_sparse")
+
 
 SCAN_CHUNK = 32          # tokens of a chunk of the chunked scan (MF_SCAN_CHUNK in csrc/recurrence.hip)
 
