@@ -26,6 +26,8 @@ OPTIONS:
   --config <FILE>         config.json to use with --random-weights
   --weight-seed <N>       seed of the random weights (default 0)
   --dtype <T>             bfloat16 (default) or float32
+  --weights <W>           stored (default), or mx4: the matrices of attention, feed-forwards and
+                          experts in microscaled 4-bit numbers (bfloat16 only)
   --temp <T>              temperature of the draw; below 1e-6 the largest logit is taken
                           (default 0.8)
   --greedy                the same as --temp 0
@@ -73,12 +75,12 @@ def parse_prompts(text: str) -> List[List[int]]:
 
 def parse_args(argv: List[str]) -> dict:
     o = dict(model=None, prompt_tokens=None, random_weights=False, config=None, weight_seed=0,
-             dtype="bfloat16", temp=0.8, top_k=40, top_p=0.95, repeat_penalty=1.1, frequency_penalty=0.0,
+             dtype="bfloat16", weights="stored", temp=0.8, top_k=40, top_p=0.95, repeat_penalty=1.1, frequency_penalty=0.0,
              presence_penalty=0.0, stop_tokens=None, n_predict=512, seed=42, n_ctx=4096, n_slots=None,
              graph=True, help=False, version=False)
     valued = {
         "--prompt-tokens": ("prompt_tokens", str), "--config": ("config", str),
-        "--weight-seed": ("weight_seed", int), "--dtype": ("dtype", str), "--temp": ("temp", float),
+        "--weight-seed": ("weight_seed", int), "--dtype": ("dtype", str), "--weights": ("weights", str), "--temp": ("temp", float),
         "-t": ("temp", float), "--top-k": ("top_k", int), "--top-p": ("top_p", float),
         "--repeat-penalty": ("repeat_penalty", float), "--frequency-penalty": ("frequency_penalty", float),
         "--presence-penalty": ("presence_penalty", float), "-n": ("n_predict", int),
@@ -133,6 +135,10 @@ def main(argv: Optional[List[str]] = None, prog: str = "minfer") -> int:
             return 0
         if o["dtype"] not in ("bfloat16", "bf16", "float32", "fp32"):
             raise UsageError(f"--dtype: {o['dtype']!r} is not bfloat16 or float32")
+        if o["weights"] not in ("stored", "mx4"):
+            raise UsageError(f"--weights: {o['weights']!r} is not stored or mx4")
+        if o["weights"] == "mx4" and o["dtype"] not in ("bfloat16", "bf16"):
+            raise UsageError("--weights mx4 runs with --dtype bfloat16")
         if o["prompt_tokens"] is None:
             raise UsageError("--prompt-tokens is required")
         if o["model"] is None and not (o["random_weights"] and o["config"]):
@@ -149,7 +155,7 @@ def main(argv: Optional[List[str]] = None, prog: str = "minfer") -> int:
     n_slots = o["n_slots"] or min(len(prompts), 64)
     try:
         llm = LLM(o["model"], config=o["config"], random_weights=o["random_weights"],
-                  weight_seed=o["weight_seed"], dtype=o["dtype"], n_ctx=o["n_ctx"], n_slots=n_slots)
+                  weight_seed=o["weight_seed"], dtype=o["dtype"], weights=o["weights"], n_ctx=o["n_ctx"], n_slots=n_slots)
         res = llm.generate(prompts, max_new=o["n_predict"], temp=o["temp"], top_k=o["top_k"], top_p=o["top_p"],
                            repeat_penalty=o["repeat_penalty"], frequency_penalty=o["frequency_penalty"],
                            presence_penalty=o["presence_penalty"], seed=o["seed"],

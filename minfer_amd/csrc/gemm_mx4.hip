@@ -16,6 +16,9 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
 }
 
+// the gate of a product: silu, or with a limit above 0 the clamped form
+__device__ __forceinline__ float gate_mul(float g, float u, float limit) { return limit > 0.f ? clamped_gate(g, u, limit) : silu_mul(g, u); }
+
 // one value of a result that is not gated
 __device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float v, int epi) {
   if (epi == EPI_BF16) ((bf16*)C)[at] = (bf16)v;
@@ -59,7 +62,8 @@ struct Rows6 { const unsigned char* codes; const unsigned* powers; };
 template <typename XT, bool VEC, int MT, int R, int NW, int D, bool PAIR>
 __global__ __launch_bounds__(NW * 64) void few_kernel(const XT* __restrict__ x, Rows6 six, const uint4* __restrict__ codes,
                                                       const unsigned* __restrict__ powers, const float* __restrict__ bias,
-                                                      void* __restrict__ C, int M, int N, int K, int tiles, int steps, int groups, int epi) {
+                                                      void* __restrict__ C, int M, int N, int K, int tiles, int steps, int groups, int epi,
+                                                      float limit) {
   constexpr bool RAW = !std::is_same<XT, void>::value;            // x as it comes, or in E2M3
   constexpr int W = RAW ? (std::is_same<XT, float>::value ? 32 : 16) : 1;
   static_assert(!RAW || MT == 1, "rows as they come: at most 16");
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(const XT* __restrict__ x, 
           gate += red[q][e / OUT][at];
           up += red[q][e / OUT][at + 16];
         }
-        if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)silu_mul(gate, up);
+        if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)gate_mul(gate, up, limit);
       } else {
         const int n = tile0 * 16 + c;
         float v = 0.f;
@@ -264,7 +268,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
                                                       const unsigned char* __restrict__ w_codes, const unsigned char* __restrict__ w_powers,
                                                       const float* __restrict__ bias, void* __restrict__ C, float* __restrict__ part, int M,
                                                       int N, int m32, int w16, int steps, int groups, int tiles_m, int tiles_n,
-                                                      int groups_per_part, int epi) {
+                                                      int groups_per_part, int epi, float limit) {
   using TT = Tile<BM, BN, STAGES>;
   constexpr int I = TT::I, J = TT::J;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -442,7 +446,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
         for (int q = 0; q < 2; ++q) {
           bf16x4 y;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) y[x] = (bf16)silu_mul(acc[i][j][4 * q + x], acc[i][j][8 + 4 * q + x]);
+          for (int x = 0; x < 4; ++x) y[x] = (bf16)gate_mul(acc[i][j][4 * q + x], acc[i][j][8 + 4 * q + x], limit);
           *reinterpret_cast<bf16x4*>(own + l32 * TT::ROW + (j * 16 + q * 8 + half * 4) * 2) = y;
         }
       __builtin_amdgcn_wave_barrier();
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
 
 // The parts of a product whose K was cut, added in their order.  A thread takes four neighbouring matrix rows of one row.
 __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ part, const float* __restrict__ bias, void* __restrict__ C, int M,
-                                                    int N, int width, int splits, int epi) {
+                                                    int N, int width, int splits, int epi, float limit) {
   const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, stride = (size_t)M * width;
   const int per = (epi == EPI_SWIGLU ? width / 2 : width) / 4;
   const int m = (int)(at / per), c = (int)(at - (size_t)m * per) * 4;
@@ -491,7 +495,7 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
   };
   if (epi == EPI_SWIGLU) {
     const float4 g = sum((c >> 4) * 32 + (c & 15)), u = sum((c >> 4) * 32 + 16 + (c & 15));
-    const float y[4] = {silu_mul(g.x, u.x), silu_mul(g.y, u.y), silu_mul(g.z, u.z), silu_mul(g.w, u.w)};
+    const float y[4] = {gate_mul(g.x, u.x, limit), gate_mul(g.y, u.y, limit), gate_mul(g.z, u.z, limit), gate_mul(g.w, u.w, limit)};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (c + i < N) ((bf16*)C)[(size_t)m * N + c + i] = (bf16)y[i];
@@ -547,33 +551,33 @@ MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int n_cu, long long* out
 
 template <int BM, int BN, int STAGES, int PER_CU, bool PAIR>
 static int launch_tiles(const unsigned char* six, const void* codes, const void* powers, const float* bias, void* C, float* part, int M, int N,
-                        int m32, int w16, int steps, int groups, const Plan& p, int epi, hipStream_t stream) {
+                        int m32, int w16, int steps, int groups, const Plan& p, int epi, float limit, hipStream_t stream) {
   using TT = Tile<BM, BN, STAGES>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<BM, BN, STAGES, PER_CU, PAIR>), hipFuncAttributeMaxDynamicSharedMemorySize, TT::LDS);
   if (e != hipSuccess) return (int)e;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (w16 * 16 + BN - 1) / BN;
   tile_kernel<BM, BN, STAGES, PER_CU, PAIR><<<dim3(tiles_m * tiles_n, p.splits), 256, TT::LDS, stream>>>(
       six, six + (size_t)m32 * steps * 3072, (const unsigned char*)codes, (const unsigned char*)powers, bias, C, p.splits > 1 ? part : nullptr, M, N,
-      m32, w16, steps, groups, tiles_m, tiles_n, p.groups, epi);
+      m32, w16, steps, groups, tiles_m, tiles_n, p.groups, epi, limit);
   return mf_launch_status();
 }
 
 template <typename XT, bool VEC, int MT, int D>
 static int launch_few(const XT* x, const Rows6& six, const void* codes, const void* powers, const float* bias, void* C, int M, int N, int K, int w16,
-                      int steps, int groups, int epi, hipStream_t stream) {
+                      int steps, int groups, int epi, float limit, hipStream_t stream) {
   if (epi == EPI_SWIGLU)
     few_kernel<XT, VEC, MT, 2, 8, D, true><<<(w16 + 1) / 2, 512, 0, stream>>>(x, six, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K,
-                                                                            w16, steps, groups, epi);
+                                                                            w16, steps, groups, epi, limit);
   else
     few_kernel<XT, VEC, MT, 1, 8, D, false><<<w16, 512, 0, stream>>>(x, six, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K, w16,
-                                                                     steps, groups, epi);
+                                                                     steps, groups, epi, limit);
   return mf_launch_status();
 }
 
 // C [M][N] (float32, added to where epi is EPI_ACC_F32, or bfloat16) from x [M][K] (bfloat16 or float32) and the stored [N][K]; EPI_SWIGLU: C is
-// [M][N] bfloat16 and the matrix holds N gate rows and N up rows, tile by tile in turn.  scratch: as `mf_mx4_plan` says, 16-byte aligned.
+// [M][N] bfloat16 and the matrix holds N gate rows and N up rows, tile by tile in turn (limit above 0: the clamped gate with it).  scratch: as `mf_mx4_plan` says, 16-byte aligned.
 MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const void* powers, const float* bias, void* C, void* scratch, float* part,
-                         int M, int N, int K, int epi, int n_cu, hipStream_t stream) {
+                         int M, int N, int K, int epi, float limit, int n_cu, hipStream_t stream) {
   long long sizes[4];
   const int bad = mf_mx4_plan(M, N, K, epi == EPI_SWIGLU, n_cu, sizes);
   if (bad) return bad;
@@ -585,7 +589,7 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
     auto run = [&](auto T0, auto VEC) {
       using T = decltype(T0);
       return launch_few<T, decltype(VEC)::value, 1, sizeof(T) == 2 ? 4 : 2>((const T*)x, six, codes, powers, bias, C, M, N, K, w16, steps, groups,
-                                                                          epi, stream);
+                                                                          epi, limit, stream);
     };
     if (is_bf16) return vec ? run(bf16{}, std::true_type{}) : run(bf16{}, std::false_type{});
     return vec ? run(float{}, std::true_type{}) : run(float{}, std::false_type{});
@@ -603,14 +607,14 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
   if (rc) return rc;
   if (p.form == FEW_SIX) {
     auto run = [&](auto MT) {
-      return launch_few<void, true, decltype(MT)::value, 4>((const void*)nullptr, six, codes, powers, bias, C, M, N, K, w16, steps, groups, epi, stream);
+      return launch_few<void, true, decltype(MT)::value, 4>((const void*)nullptr, six, codes, powers, bias, C, M, N, K, w16, steps, groups, epi, limit, stream);
     };
     if (M <= 32) return run(std::integral_constant<int, 2>{});
     return run(std::integral_constant<int, 4>{});
   }
   auto tiles = [&](auto BM, auto BN, auto STAGES, auto PER_CU, auto PAIR) {
     return launch_tiles<decltype(BM)::value, decltype(BN)::value, decltype(STAGES)::value, decltype(PER_CU)::value, decltype(PAIR)::value>((const unsigned char*)scratch, codes, powers, bias, C, part, M, N,
-                                                                                     m32, w16, steps, groups, p, epi, stream);
+                                                                                     m32, w16, steps, groups, p, epi, limit, stream);
   };
   auto choose = [&](auto PAIR) {
     using std::integral_constant;
@@ -623,6 +627,6 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
   rc = epi == EPI_SWIGLU ? choose(std::true_type{}) : choose(std::false_type{});
   if (rc || p.splits == 1) return rc;
   const size_t per = (size_t)(epi == EPI_SWIGLU ? w16 * 8 : w16 * 16) / 4;
-  parts_kernel<<<(unsigned)((per * M + 255) / 256), 256, 0, stream>>>(part, bias, C, M, N, w16 * 16, p.splits, epi);
+  parts_kernel<<<(unsigned)((per * M + 255) / 256), 256, 0, stream>>>(part, bias, C, M, N, w16 * 16, p.splits, epi, limit);
   return mf_launch_status();
 }

@@ -70,15 +70,16 @@ def tensor_shapes(folder: str) -> Dict[str, Tuple[int, ...]]:
         raise WeightError(str(e)) from None
 
 
-def load_model(folder: str, dtype="bfloat16", device="cuda:0") -> DecoderModel:
+def load_model(folder: str, dtype="bfloat16", device="cuda:0", weights: str = "stored") -> DecoderModel:
     """config.json picks the architecture; model.safetensors gives the tensors by name.  Stop
-    tokens are config.json's, joined by generation_config.json's where the folder has one."""
+    tokens are config.json's, joined by generation_config.json's where the folder has one.  `weights` "mx4": the matrices of the
+    parts that know how are kept in microscaled 4-bit numbers, made as they are loaded."""
     device = require_gpu(device)
     config = config_from_dict(read_config_json(folder))
     if hasattr(config, "adopt_tensor_shapes"):
         # a design may leave a size to its tensors (the rows of a table): the configuration takes it from the file
         config.adopt_tensor_shapes(tensor_shapes(folder))
-    model = DecoderModel(config.model_spec(), run_dtype(dtype), device)
+    model = DecoderModel(config.model_spec(), run_dtype(dtype), device, weights)
     model.config = config
     expected = model.expected_tensors()
     # tensors a file may hold without the model wanting them (a stored copy of a tied head)
@@ -95,16 +96,16 @@ def load_model(folder: str, dtype="bfloat16", device="cuda:0") -> DecoderModel:
 
 
 def random_model(config: Union[Dict[str, Any], Any], seed: int = 0, dtype="bfloat16",
-                 device="cuda:0") -> DecoderModel:
+                 device="cuda:0", weights: str = "stored") -> DecoderModel:
     """Random weights made on the device (no file): the tensors that `write_random_model` writes
     for the same configuration and seed (in bfloat16) and `load_model` reads back, value for
     value: matrices, tables and biases N(0, std of the configuration) rounded to bfloat16, norm
-    gains one; a tensor's values depend on (seed, its name, the index)."""
+    gains one; a tensor's values depend on (seed, its name, the index).  `weights` as `load_model` takes it."""
     device = require_gpu(device)
     if isinstance(config, dict):
         config = config_from_dict(config)
     dt = run_dtype(dtype)
-    model = DecoderModel(config.model_spec(), dt, device)
+    model = DecoderModel(config.model_spec(), dt, device, weights)
     model.config = config
     expected = model.expected_tensors()
 

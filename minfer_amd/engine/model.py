@@ -21,6 +21,10 @@ from ..weights.loader import TensorSpec
 from .alike import MOST_VALUES, AlikeLayers
 
 
+# how the matrices are kept: as they are stored, or ("mx4") those of the parts that know how in microscaled 4-bit numbers
+WEIGHTS = ("stored", "mx4")
+
+
 def _build_block(bs: BlockSpec, rt: Runtime):
     """The block's arrangement and the parts its spec names; the arrangement says which it needs."""
     if bs.kind not in BLOCKS:
@@ -48,17 +52,23 @@ def _build_block(bs: BlockSpec, rt: Runtime):
 
 
 class DecoderModel:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, weights: str = "stored"):
+        if weights not in WEIGHTS:
+            raise ValueError(f"weights must be one of {', '.join(WEIGHTS)}, got {weights!r}")
+        if weights == "mx4" and dtype != torch.bfloat16:
+            raise ValueError("weights 'mx4' run with bfloat16 activations; the float32 run type takes its weights as they are stored")
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"run type must be float32 or bfloat16, got {dtype}")
         self.spec = spec
-        self.rt = Runtime(dtype=dtype, device=torch.device(device))
+        self.rt = Runtime(dtype=dtype, device=torch.device(device), mx4=weights == "mx4")
         self.blocks = [_build_block(bs, self.rt) for bs in spec.blocks]
         self.final_norm = make_part(NORMS, spec.final_norm, self.rt, "norm")
         self.embedding = make_part(EMBEDDINGS, spec.embedding, self.rt, "embedding")
         self.head = make_part(HEADS, spec.head, self.rt, "head")
         if self.embedding.cache_request() is not None and any(e.adds_embedding for e in spec.schedule):
             raise ValueError("an embedding that keeps state runs once a step; this run order takes its output in again")
+        if self.rt.mx4 and not any(part.knows_mx4 for block in self.blocks for part in block.parts()):
+            raise ValueError("weights 'mx4': no part of this model keeps its matrices in microscaled 4-bit numbers")
         self.stop_tokens = tuple(spec.stop_tokens)      # a loader may add to them (generation_config.json)
         self.loaded = False
         self.decode_copy_bytes = 0      # of the parts' tiled second copies, once loaded

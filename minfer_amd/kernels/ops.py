@@ -163,7 +163,7 @@ _PROTOTYPES = {
     },
     "gemm_mx4": {
         "mf_mx4_plan": [c_int, c_int, c_int, c_int, c_int, _P],
-        "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P],
+        "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, c_int, _P],
     },
     "moe_mx4": {
         "mf_mx4_moe": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
@@ -2257,7 +2257,7 @@ def _mx4_plan(m: int, n: int, k: int, swiglu: bool, n_cu: int) -> Tuple[int, int
 
 
 def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
-                 epi: int) -> None:
+                 epi: int, limit: float = 0.0) -> None:
     m, k = x.shape
     n = out.shape[1]
     if m == 0:
@@ -2267,7 +2267,7 @@ def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.
     _, _, six, parts = _mx4_plan(m, n, k, epi == EPI_SWIGLU, n_cu)
     scratch = torch.empty(six, dtype=torch.uint8, device=x.device) if six else None
     part = torch.empty(parts, dtype=torch.float32, device=x.device) if parts else None
-    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, n_cu, _stream()),
+    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, limit, n_cu, _stream()),
            f"{what} {m}x{n}x{k}")
 
 
@@ -2301,9 +2301,11 @@ def mx4_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return torch.stack([gate, up], dim=-4).flatten(-5, -4).contiguous()
 
 
-def mx4_linear_swiglu(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor) -> None:
+def mx4_linear_swiglu(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor, limit: float = 0.0) -> None:
     """out = silu(x' G'^T) * (x' U'^T), rounded once to bfloat16, in one product; `codes`, `powers`: `mx4_pairs` of those of G and U `[f][k]`;
-    x' as in `mx4_linear`, `out` bfloat16 `[m][f]`."""
+    x' as in `mx4_linear`, `out` bfloat16 `[m][f]`.  A `limit` above 0: the clamped form of `swiglu` with it."""
+    if limit < 0:
+        raise KernelError(f"mx4_linear_swiglu: limit {limit}")
     _need(x, "mx4_linear_swiglu.x", _FLOATS)
     _need(out, "mx4_linear_swiglu.out", torch.bfloat16)
     if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0]:
@@ -2313,7 +2315,7 @@ def mx4_linear_swiglu(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor
     (tiles, *c), (_, *p) = mx4_shapes(f, k)
     _need(codes, "mx4_linear_swiglu.codes", torch.uint8, (2 * tiles, *c))
     _need(powers, "mx4_linear_swiglu.powers", torch.uint8, (2 * tiles, *p))
-    _mx4_product("mx4_linear_swiglu", x, codes, powers, None, out, EPI_SWIGLU)
+    _mx4_product("mx4_linear_swiglu", x, codes, powers, None, out, EPI_SWIGLU, float(limit))
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

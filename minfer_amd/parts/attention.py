@@ -14,7 +14,7 @@ from ..cache.paged import KVRequest
 from ..kernels import ops
 from ..weights.loader import TensorSpec
 from .base import Mixer, POSITIONS, make_part, register_mixer
-from .linear import Linear
+from .linear import linear_class
 from .rotary import RotaryNeoX
 
 
@@ -22,6 +22,8 @@ from .rotary import RotaryNeoX
 class GQAttention(Mixer):
     """params: hidden_size, n_heads, n_kv_heads, head_dim, scale, window (None or int),
     qkv_bias, out_bias, position (PartSpec), q/k/v/o (tensor name stems)."""
+
+    knows_mx4 = True
 
     def __init__(self, spec, rt):
         super().__init__(spec, rt)
@@ -57,8 +59,9 @@ class GQAttention(Mixer):
         n = self.names
         ws = [get(n[k] + ".weight") for k in ("q", "k", "v")]
         bs = [get(n[k] + ".bias") for k in ("q", "k", "v")] if self.qkv_bias else None
-        self.qkv = Linear.stacked(ws, bs)
-        self.o = Linear(get(n["o"] + ".weight"), get(n["o"] + ".bias") if self.out_bias else None)
+        kind = linear_class(self.rt)
+        self.qkv = kind.stacked(ws, bs)
+        self.o = kind(get(n["o"] + ".weight"), get(n["o"] + ".bias") if self.out_bias else None)
 
     def cache_request(self):
         return KVRequest(self.nk, self.hd, None if self.window is None else int(self.window))

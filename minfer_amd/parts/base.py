@@ -26,6 +26,7 @@ class Runtime:
     """Where and in which precision a model runs."""
     dtype: torch.dtype          # run type of activations, matrices and cache
     device: torch.device
+    mx4: bool = False           # parts that know how (`Part.knows_mx4`) keep their matrices in microscaled 4-bit numbers
 
     @property
     def is_bf16(self) -> bool:
@@ -37,6 +38,8 @@ class Part:
 
     def __init__(self, spec: PartSpec, rt: Runtime):
         self.spec, self.rt = spec, rt
+
+    knows_mx4 = False            # whether the part's matrices become microscaled 4-bit ones under `Runtime.mx4`
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         return {}

@@ -10,7 +10,7 @@ import torch
 from ..kernels import ops
 from ..weights.loader import TensorSpec
 from .base import FeedForward, Normed, register_feed_forward
-from .linear import Linear
+from .linear import Linear, linear_class, mx4_gate_up
 
 
 @register_feed_forward("swiglu")
@@ -21,6 +21,7 @@ class SwiGLU(FeedForward):
     ".weight"), limit (None, or a positive number)."""
 
     can_overwrite = True
+    knows_mx4 = True
 
     def __init__(self, spec, rt):
         super().__init__(spec, rt)
@@ -30,7 +31,7 @@ class SwiGLU(FeedForward):
         self.limit = None if p.get("limit") is None else float(p["limit"])
         if self.limit is not None and not self.limit > 0:
             raise ValueError(f"swiglu: limit {self.limit} must be positive")
-        self.gate_up = self.down = self.fused = self.fused_tiled = self.limit_on_device = None
+        self.gate_up = self.down = self.fused = self.fused_tiled = self.limit_on_device = self.mx4 = None
 
     def tensor_specs(self):
         n = self.names
@@ -40,13 +41,16 @@ class SwiGLU(FeedForward):
     def load(self, get):
         n = self.names
         gate, up = get(n["gate"]), get(n["up"])
-        if self.rt.is_bf16 and gate.dtype == up.dtype == torch.bfloat16:
+        if self.rt.mx4:
+            self.mx4 = mx4_gate_up(gate, up)
+        elif self.rt.is_bf16 and gate.dtype == up.dtype == torch.bfloat16:
             self.fused = ops.interleave_gate_up(gate, up)
         else:
             self.gate_up = Linear.stacked([gate, up])
-        self.down = Linear(get(n["down"]))
+        down = get(n["down"])
+        self.down = linear_class(self.rt)(down)
         if self.limit is not None:
-            self.limit_on_device = torch.tensor([self.limit], dtype=torch.float32, device=self.down.weight.device)
+            self.limit_on_device = torch.tensor([self.limit], dtype=torch.float32, device=down.device)
 
     def decode_copies(self, make: bool, min_row_length: int = 0) -> int:
         n = self.down.decode_copy(make, min_row_length)
@@ -64,12 +68,14 @@ class SwiGLU(FeedForward):
     def alike(self):
         if type(self) is not SwiGLU:
             return None
-        gate_up = (None, None, None) if self.gate_up is None else self.gate_up.tensors()
+        gate_up = self.mx4 + (None,) if self.mx4 is not None else (None, None, None) if self.gate_up is None else self.gate_up.tensors()
         return (SwiGLU, self.hidden, self.inter, self.limit), (self.fused, self.fused_tiled, self.limit_on_device) + gate_up + self.down.tensors()
 
     def forward(self, x, h, ctx, accumulate: bool = True) -> None:
         y = torch.empty((x.shape[0], self.inter), dtype=self.rt.dtype, device=x.device)
-        if self.fused is not None:
+        if self.mx4 is not None:
+            ops.mx4_linear_swiglu(x.tensor() if isinstance(x, Normed) else x, *self.mx4, y, limit=self.limit or 0.0)
+        elif self.fused is not None:
             # (the clamped form has no fold of the norm before it)
             fold = x.norm.rms_scale() if isinstance(x, Normed) and self.limit is None else None
             done = False

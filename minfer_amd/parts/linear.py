@@ -19,6 +19,11 @@ def common_matrix_dtype(tensors: List[torch.Tensor]) -> torch.dtype:
     return torch.bfloat16 if all(t.dtype == torch.bfloat16 for t in tensors) else torch.float32
 
 
+def linear_class(rt):
+    """What a part that knows microscaled matrices makes its own of."""
+    return MX4Linear if rt.mx4 else Linear
+
+
 class Linear:
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
         if weight.dim() != 2:
@@ -133,3 +138,44 @@ class Linear:
             return False
         ctx.norm_ahead = NormAhead(norm, out, xg, sums)
         return True
+
+
+class MX4Linear(Linear):
+    """A matrix in microscaled 4-bit numbers (`ops.mx4_quantise`), made from the one that is loaded, which is not kept: 17/32 of a byte a value.
+    Its rows of activations meet it in microscaled 6-bit ones, which the product makes on its way (`ops.mx4_linear`); biases and sums are
+    32-bit as ever.  No norm is folded into such a product and none prepared behind it."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        super().__init__(weight, bias)
+        self.codes, self.powers = mx4_matrix(self.weight)
+        self.weight = None
+
+    def tensors(self):
+        return self.codes, self.powers, self.bias
+
+    def decode_copy(self, make: bool, min_row_length: int = 0) -> int:
+        return 0
+
+    def __call__(self, x, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32, accumulate: bool = False,
+                 ctx=None) -> torch.Tensor:
+        if isinstance(x, Normed):
+            x = x.tensor()
+        if out is None:
+            out = torch.empty((x.shape[0], self.out_features), dtype=out_dtype, device=x.device)
+        ops.mx4_linear(x, self.codes, self.powers, self.bias, out, accumulate=accumulate)
+        return out
+
+    def parts(self, x):
+        return None
+
+
+def mx4_matrix(weight: torch.Tensor):
+    """(codes, powers) of a matrix `[rows][k]`."""
+    codes, powers = (torch.empty(s, dtype=torch.uint8, device=weight.device) for s in ops.mx4_shapes(*weight.shape))
+    ops.mx4_quantise(weight, codes, powers)
+    return codes, powers
+
+
+def mx4_gate_up(gate: torch.Tensor, up: torch.Tensor):
+    """(codes, powers) of gate and up matrices as `ops.mx4_linear_swiglu` reads them."""
+    return tuple(ops.mx4_pairs(g, u) for g, u in zip(mx4_matrix(gate), mx4_matrix(up)))

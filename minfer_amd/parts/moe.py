@@ -30,6 +30,9 @@ allow it, `ops.linear_grouped`, else an expert at a time), and the rows' results
 added into the stream with the tokens' weights, a token's choices in their order.  (With a table nothing waits:
 the host counts the experts' pairs itself.)
 
+With `Runtime.mx4` the experts' matrices are kept in microscaled 4-bit numbers: few tokens take `ops.mx4_moe_sparse`, many two products an
+expert over its tokens' rows (`ops.mx4_linear_swiglu`, `ops.mx4_linear`).  Router, table and the shared expert stay as they are.
+
 A step whose context carries a list under `_memo["route_log"]` gets every routed layer's choices
 (`[rows][top]` expert numbers, on the device) appended to it, in run order.
 """
@@ -41,7 +44,7 @@ import torch
 from ..kernels import ops
 from ..weights.loader import TensorSpec, WeightError
 from .base import FeedForward, register_feed_forward
-from .linear import Linear
+from .linear import Linear, mx4_gate_up, mx4_matrix
 
 # steps of at most this many tokens read only the chosen experts' matrices
 SPARSE_UP_TO = ops.MOE_SPARSE_TOKENS
@@ -96,6 +99,7 @@ class Experts(FeedForward):
     numbers from n_experts on stand for experts that hand their input on; default 0)."""
 
     can_overwrite = True
+    knows_mx4 = True
 
     def __init__(self, spec, rt):
         super().__init__(spec, rt)
@@ -114,7 +118,7 @@ class Experts(FeedForward):
         if self.ne < 1 or self.identity < 0 or not 1 <= self.top <= min(64, self.choices) or self.choices > ops.MOE_MAX_EXPERTS:
             raise ValueError(f"{spec.kind}: {self.top} of {self.ne} + {self.identity} experts chosen (at most 64 of at most "
                              f"{ops.MOE_MAX_EXPERTS})")
-        self.gate_up = self.down = None
+        self.gate_up = self.down = self.mx4 = None
 
     def tensor_specs(self):
         s = {}
@@ -129,6 +133,14 @@ class Experts(FeedForward):
 
     def load(self, get):
         stems = [self.expert_name.format(e) for e in range(self.ne)]
+        if self.rt.mx4:
+            # gate|up codes and powers, down codes and powers, each of all experts
+            gate_up = [mx4_gate_up(get(s + ".gate"), get(s + ".up")) for s in stems]
+            down = [mx4_matrix(get(s + ".down")) for s in stems]
+            self.mx4 = tuple(torch.stack([t[i] for t in made]) for made in (gate_up, down) for i in (0, 1))
+            if self.shared is not None:
+                self.shared.load(get)
+            return
         # [experts][gate | up][hidden] and [experts][hidden][inter]: an expert's matrices are contiguous slices
         self.gate_up = torch.stack([torch.cat([get(s + ".gate"), get(s + ".up")], dim=0) for s in stems]).contiguous()
         self.down = torch.stack([get(s + ".down") for s in stems]).contiguous()
@@ -161,7 +173,12 @@ class Experts(FeedForward):
             self.shared.forward(x, h, accumulate)
             accumulate = True
         few = min(SPARSE_UP_TO, max(1, ops.MOE_SPARSE_PAIRS // self.top))
-        if (n <= few or (ctx is not None and ctx.all_decode)) and x.dtype == self.gate_up.dtype:
+        if self.mx4 is not None and (n <= few or (ctx is not None and ctx.all_decode)):
+            for t0 in range(0, n, few):
+                ops.mx4_moe_sparse(x[t0:t0 + few], *self.mx4, chosen[t0:t0 + few], weights[t0:t0 + few], h[t0:t0 + few], self.inter, self.limit,
+                                   self.act, accumulate=accumulate, hands_on=self.identity > 0)
+            return
+        if self.mx4 is None and (n <= few or (ctx is not None and ctx.all_decode)) and x.dtype == self.gate_up.dtype:
             for t0 in range(0, n, few):      # (slices of a contiguous tensor's rows are contiguous)
                 ops.moe_sparse(x[t0:t0 + few], self.gate_up, self.down, chosen[t0:t0 + few], weights[t0:t0 + few],
                                h[t0:t0 + few], self.ne, self.limit, self.act, accumulate=accumulate, hands_on=self.identity > 0)
@@ -178,7 +195,7 @@ class Experts(FeedForward):
         pairs = starts[-1]                   # of experts with matrices; the others' stand nowhere
         handed = dict(x=x, n_real=self.ne) if self.identity else {}
         # one product over all experts' rows where its kernel takes the sizes, else a product an expert
-        grouped = pairs > 0 and x.dtype == self.gate_up.dtype and ops.grouped_takes(x.dtype, 2 * self.inter, self.hidden) \
+        grouped = self.mx4 is None and pairs > 0 and x.dtype == self.gate_up.dtype and ops.grouped_takes(x.dtype, 2 * self.inter, self.hidden) \
             and ops.grouped_takes(x.dtype, self.hidden, self.inter)
         plans = [ops.grouped_plan(per_expert, 2 * self.inter, self.hidden), ops.grouped_plan(per_expert, self.hidden, self.inter)] \
             if grouped else []
@@ -198,6 +215,13 @@ class Experts(FeedForward):
             up_groups, down_groups = (meta[at + o:at + o + s].view(-1, 4) for o, s in zip((0, sizes[0]), sizes))
             ops.linear_grouped_gated(xs, self.gate_up, up_groups, plans[0], y, self.limit, self.act)
             ops.linear_grouped(y, self.down, down_groups, plans[1], rows)
+        elif self.mx4 is not None:
+            gate_up, gate_up_powers, down, down_powers = self.mx4
+            for e in range(self.ne):
+                if per_expert[e]:
+                    mine = slice(starts[e], starts[e + 1])
+                    ops.mx4_linear_swiglu(xs[mine], gate_up[e], gate_up_powers[e], y[mine], limit=0.0 if self.act else self.limit)
+                    ops.mx4_linear(y[mine], down[e], down_powers[e], None, rows[mine])
         else:
             gu = torch.empty((pairs, 2 * self.inter), dtype=torch.float32, device=dev)
             for e, (gate_up, _) in enumerate(self.experts):

@@ -127,6 +127,21 @@ def test_linear_swiglu(m, f, k):
     within(out, want, bound + half_step(BF16) * (want.abs() + bound) + 1e-37)
 
 
+@pytest.mark.parametrize("m", [7, 48, 130])
+def test_linear_swiglu_clamped(m):
+    from minfer_amd.kernels import ops
+    f, k, limit = 90, 260, 0.7
+    x = normal((m, k), m)
+    gate, up = quantised(normal((f, k), 1, std=0.05)), quantised(normal((f, k), 2, std=0.05))
+    out = torch.full((m, f), float("nan"), dtype=BF16, device=DEV)
+    ops.mx4_linear_swiglu(x, ops.mx4_pairs(gate[0], up[0]), ops.mx4_pairs(gate[1], up[1]), out, limit=limit)
+    (g, g_size), (u, u_size) = (plain.product(x, plain.read(*t, f, k)) for t in (gate, up))
+    want = plain.act(g, u, limit, 0)
+    # the gate's slope is below 1.2 and itself below the limit, u + 1 at most limit + 1
+    bound = 1.2 * (limit + 1) * plain.sum_error(k, g_size) + limit * plain.sum_error(k, u_size) + (g.abs() + 16) * 2.0 ** -22 * (limit + 1)
+    within(out, want, bound + half_step(BF16) * (want.abs() + bound))
+
+
 def test_rows_apart():
     """An infinity or a NaN in a row of x makes that row NaN and no other; a NaN block of the matrix makes its output NaN in every row."""
     from minfer_amd.kernels import ops
