@@ -62,6 +62,8 @@ def parse():
     ap.add_argument("--shape", default="7b", choices=list(SHAPES), help="layer sizes (default: Qwen2.5-7B)")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers than the model has")
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "mx4"],
+                    help="mx4: the matrices of attention and feed-forwards in microscaled 4-bit numbers (bf16 only)")
     ap.add_argument("--no-points", action="store_true", help="skip the further points (batch 1 and 64, long contexts, other prefills)")
     ap.add_argument("--breakdown", action="store_true", help="time every kernel of one decode step (batch of --batch)")
     ap.add_argument("--max-tokens", type=int, default=None,
@@ -88,11 +90,11 @@ def matrix_params(cfg):
     return per_layer, small, cfg["vocab_size"] * h
 
 
-def decode_bytes(cfg, elem, total_context):
+def decode_bytes(cfg, elem, total_context, matrix_elem=None):
     per_layer, small, head = matrix_params(cfg)
     nk, hd = cfg["num_key_value_heads"], cfg.get("head_dim") or cfg["hidden_size"] // cfg["num_attention_heads"]
     L = cfg["num_hidden_layers"]
-    weights = (L * per_layer + head) * elem + (L * small + cfg["hidden_size"]) * 4
+    weights = L * per_layer * (matrix_elem or elem) + head * elem + (L * small + cfg["hidden_size"]) * 4
     kv = total_context * 2 * L * nk * hd * elem
     return weights + kv
 
@@ -218,7 +220,8 @@ def run_decode(eng, cfg, batch, prompt_max, steps, warmup, use_graph, elem, seed
     ctx_end = sum(eng.length(s) for s in slots)
     for s in slots:
         eng.end_sequence(s)
-    nbytes = (bytes_fn or decode_bytes)(cfg, elem, (ctx_start + ctx_end) / 2.0)
+    matrix = {} if bytes_fn or not eng.model.rt.mx4 else dict(matrix_elem=17 / 32)
+    nbytes = (bytes_fn or decode_bytes)(cfg, elem, (ctx_start + ctx_end) / 2.0, **matrix)
     return dict(tok_s=batch * steps / dt, ms=dt / steps * 1e3, gbs=nbytes / (dt / steps) / 1e9, bytes=nbytes)
 
 
@@ -485,7 +488,7 @@ def main() -> int:
     batches = [a.batch] + ([1, 64] if points_on else [])
     read_gbs, mfma_flops = measure_peaks()
     # the cache: the batch's contexts, or what the memory left by the weights holds if that is less
-    llm = LLM(config=cfg, random_weights=True, weight_seed=0, dtype=dtype, n_ctx=a.context,
+    llm = LLM(config=cfg, random_weights=True, weight_seed=0, dtype=dtype, weights=a.weights, n_ctx=a.context,
               n_slots=max(batches), max_tokens=a.max_tokens)
     eng = llm.engine
     plan = llm.cache_plan
@@ -528,7 +531,7 @@ def main() -> int:
             points[f"decode_b8_ctx{tag}"] = round(r["tok_s"], 1)
     flops = prefill_flops(cfg, a.prefill_tokens)
     out = {
-        "metric": f"decode tok/s, {shape_name} shape, batch {a.batch}", "value": round(main_run["tok_s"], 1),
+        "metric": f"decode tok/s, {shape_name} shape, batch {a.batch}" + ("" if a.weights == "stored" else f", {a.weights} weights"), "value": round(main_run["tok_s"], 1),
         "unit": "tokens/s", "n_gpus": 1, "steps": a.steps, "warmup": a.warmup,
         "ms_per_step": round(main_run["ms"], 4), "higher_is_better": True, "scaling": "weak",
         "vs_baseline": None, "dtype": a.dtype, "data": "synthetic",

@@ -1,7 +1,8 @@
 // Products with matrices in microscaled 4-bit numbers (`mx4.h`): out[m][n] (+)= sum_k X'[m][k] W'[n][k] (+ bias[n]), X' the rows x in E2M3.
 //
-//  * `few_kernel`: at most 16 rows as they come (quantised in registers on the way), or up to 64 in E2M3 already: the stream of W bounds it.
-//  * `tile_kernel`: more rows, in E2M3 (`rows_kernel` in front): tiles of the result, operands through LDS, optionally with K cut over blocks.
+//  * `few_kernel`: at most 16 rows as they come, quantised in registers on the way; `few_six_kernel`: up to 64, in E2M3 already: the stream of W
+//    bounds both.
+//  * `tile_kernel`: more rows, in E2M3 (`rows_kernel` makes them): tiles of the result, operands through LDS, optionally with K cut over blocks.
 //  * `parts_kernel` adds what those blocks left.
 #include <algorithm>
 #include <type_traits>
@@ -27,7 +28,9 @@ __device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float
 }
 
 // ------------------------------------------------------------------ rows in E2M3
-// A lane takes a block: a wave four rows and 512 k.  Bound by memory: 2 or 4 bytes a value read, 25/32 written.
+// A lane takes a block: a wave four rows and 512 k.  Bound by memory: 2 or 4 bytes a value read, 25/32 written.  Rows that do not begin at
+// multiples of 16 bytes come by way of LDS, 64 neighbouring values a load (value by value from the row itself, 32 loads of 64 lines each: 6.2 us
+// for 37 rows of 2,500, ROWS so).
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned* __restrict__ powers,
                                                    int m, int m32, int k, int steps, int groups) {
@@ -37,7 +40,14 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
   const int row = four * 4 + i;
   if (four * 4 >= m32 * 32) return;
   unsigned words[sizeof(T) * 8];
-  mx_load_block<VEC>(x + (size_t)min(row, m - 1) * k, group * 512 + c * 32, row < m ? k : 0, words);
+  if constexpr (VEC) {
+    mx_load_block(x + (size_t)min(row, m - 1) * k, group * 512 + c * 32, row < m ? k : 0, words);
+  } else {
+    __shared__ __attribute__((aligned(16))) T stage[4][4][512 + 16 / sizeof(T)];
+    T (*mine)[512 + 16 / sizeof(T)] = stage[threadIdx.x >> 6];
+    mx_stage_rows(x, mine, four * 4, m, k, group * 512, lane);
+    mx_load_block(&mine[i][0], c * 32, 512, words);
+  }
   unsigned power;
   const uintx6 six = mx6_block(words, power);
   const int step = group * 4 + (c >> 2), g = c & 3, r = row & 31;
@@ -53,125 +63,139 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
 }
 
 // ------------------------------------------------------------------ few rows
-// A workgroup owns R tiles of 16 matrix rows over the whole of K; its NW waves take the tiles' steps of 128 k in turn, so that at any time they
-// read neighbouring kilobytes, D steps of a wave in flight.  A step of a wave feeds the 16x16x128 instruction: A = 16 matrix rows as they are
-// stored, B = 16 rows of x, whose lane holds one block of one row: quantising it takes no other lane.  The waves' sums meet in LDS and are
-// added in the waves' order.  What bounds it is the stream of the matrix; the rows come from L2 again for every workgroup.
-struct Rows6 { const unsigned char* codes; const unsigned* powers; };
-
-template <typename XT, bool VEC, int MT, int R, int NW, int D, bool PAIR>
-__global__ __launch_bounds__(NW * 64) void few_kernel(const XT* __restrict__ x, Rows6 six, const uint4* __restrict__ codes,
-                                                      const unsigned* __restrict__ powers, const float* __restrict__ bias,
-                                                      void* __restrict__ C, int M, int N, int K, int tiles, int steps, int groups, int epi,
-                                                      float limit) {
-  constexpr bool RAW = !std::is_same<XT, void>::value;            // x as it comes, or in E2M3
-  constexpr int W = RAW ? (std::is_same<XT, float>::value ? 32 : 16) : 1;
-  static_assert(!RAW || MT == 1, "rows as they come: at most 16");
-  static_assert(!PAIR || R % 2 == 0, "gate and up tiles in pairs");
-  constexpr int COLS = 16 * R, RS = COLS + 4;
-  __shared__ __attribute__((aligned(16))) float red[NW][16][RS];
+// A workgroup owns R tiles of 16 matrix rows over the whole of K; its NW waves take the tiles' runs of G steps of 128 k in turn, so that at any
+// time they read neighbouring kilobytes, D runs of a wave in flight.  The waves' sums meet in LDS and are added in the waves' order.
+// What bounds it is the stream of the matrix; the rows come from L2 again for every workgroup.
+// The sums of 16 rows (from row m0 on) as they lie in a wave -> results: what every kernel of few rows ends with.
+template <int R, int NW, bool PAIR>
+__device__ __forceinline__ void few_results(const floatx4 (&acc)[R], float (*red)[16][16 * R + 4], void* __restrict__ C,
+                                            const float* __restrict__ bias, int m0, int M, int N, int tile0, int wid, int epi, float limit) {
+  constexpr int COLS = 16 * R, OUT = PAIR ? COLS / 2 : COLS;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile0 = blockIdx.x * R;
-  const uint4* wtile[R];
-  const unsigned* wpow[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) *reinterpret_cast<floatx4*>(&red[wid][r16][j * 16 + 4 * g]) = acc[j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 16 * OUT; e += NW * 64) {
+    const int m = m0 + e / OUT, c = e % OUT;
+    if (m >= M) break;
+    if constexpr (PAIR) {
+      const int f = tile0 * 8 + c, at = (c >> 4) * 32 + (c & 15);
+      float gate = 0.f, up = 0.f;
+#pragma unroll
+      for (int q = 0; q < NW; ++q) {
+        gate += red[q][e / OUT][at];
+        up += red[q][e / OUT][at + 16];
+      }
+      if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)gate_mul(gate, up, limit);
+    } else {
+      const int n = tile0 * 16 + c;
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < NW; ++q) v += red[q][e / OUT][c];
+      if (n < N) store_one(C, (size_t)m * N + n, bias ? v + bias[n] : v, epi);
+    }
+  }
+}
+
+// the tiles of a workgroup (past the last: that one again, whose results nobody stores)
+template <int R>
+__device__ __forceinline__ void few_tiles(const uint4* codes, const unsigned* powers, int tile0, int tiles, int steps, int groups, int lane,
+                                          const uint4* (&wtile)[R], const unsigned* (&wpow)[R]) {
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int tile = min(tile0 + j, tiles - 1);
     wtile[j] = codes + (size_t)tile * steps * 64 + lane;
     wpow[j] = powers + (size_t)tile * groups * 64 + lane;
   }
+}
+
+// At most 16 / G rows as they come, quantised in registers on the way.
+template <typename XT, int R, int NW, int D, int G, bool PAIR>
+__global__ __launch_bounds__(NW * 64) void few_kernel(const XT* __restrict__ x, const uint4* __restrict__ codes,
+                                                      const unsigned* __restrict__ powers, const float* __restrict__ bias,
+                                                      void* __restrict__ C, int M, int N, int K, int tiles, int steps, int groups, int epi,
+                                                      float limit) {
+  static_assert(!PAIR || R % 2 == 0, "gate and up tiles in pairs");
+  constexpr int ROWS = 16 / G;
+  __shared__ __attribute__((aligned(16))) float red[NW][16][16 * R + 4];
+  const int lane = threadIdx.x & 63, r16 = lane & 15;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint4* wtile[R];
+  const unsigned* wpow[R];
+  few_tiles<R>(codes, powers, blockIdx.x * R, tiles, steps, groups, lane, wtile, wpow);
+  floatx4 acc[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  // (rows past M: columns that nobody reads)
+  few_rows<XT, R, NW, D, G>(x + (size_t)min(r16 % ROWS, M - 1) * K, wtile, wpow, wid, r16 / ROWS, lane >> 4, steps, K, acc);
+  few_results<R, NW, PAIR>(acc, red, C, bias, 0, M, N, blockIdx.x * R, wid, epi, limit);
+}
+
+// At most 16 MT rows in E2M3.
+template <int MT, int R, int NW, int G, bool PAIR>
+__global__ __launch_bounds__(NW * 64) void few_six_kernel(const unsigned char* __restrict__ a_codes, const unsigned* __restrict__ a_powers,
+                                                          const uint4* __restrict__ codes, const unsigned* __restrict__ powers,
+                                                          const float* __restrict__ bias, void* __restrict__ C, int M, int N, int tiles,
+                                                          int steps, int groups, int epi, float limit) {
+  static_assert(!PAIR || R % 2 == 0, "gate and up tiles in pairs");
+  __shared__ __attribute__((aligned(16))) float red[NW][16][16 * R + 4];
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint4* wtile[R];
+  const unsigned* wpow[R];
+  few_tiles<R>(codes, powers, blockIdx.x * R, tiles, steps, groups, lane, wtile, wpow);
   floatx4 acc[MT][R];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < R; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-  uint4 w[D][R];
-  unsigned p[D][R], words[D][W], xp[D][MT];
-  uint4 x4[D][MT];
-  uint2 x2[D][MT];
-  auto load = [&](int s, int t) {
+  const int runs = (steps + G - 1) / G;
+  uint4 w[G][R], x4[G][MT];
+  uint2 x2[G][MT];
+  unsigned p[R], xp[MT];
+  auto load = [&](int run) {
+    const int t0 = min(run, runs - 1) * G;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      w[s][j] = wtile[j][(size_t)t * 64];
-      p[s][j] = wpow[j][(size_t)(t >> 2) * 64];
-    }
-    if constexpr (RAW) {
-      mx_load_block<VEC>(x + (size_t)min(r16, M - 1) * K, t * 128 + g * 32, r16 < M ? K : 0, words[s]);
-    } else {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const unsigned char* tile = six.codes + ((size_t)(i >> 1) * steps + t) * 3072;
-        const int r = (i & 1) * 16 + r16;
-        x4[s][i] = *reinterpret_cast<const uint4*>(tile + g * 512 + r * 16);
-        x2[s][i] = *reinterpret_cast<const uint2*>(tile + 2048 + g * 256 + r * 8);
-        xp[s][i] = six.powers[((size_t)(i >> 1) * groups + (t >> 2)) * 128 + g * 32 + r];
-      }
+      for (int q = 0; q < G; ++q) w[q][j] = wtile[j][(size_t)min(t0 + q, steps - 1) * 64];
+      p[j] = wpow[j][(size_t)(t0 >> 2) * 64];
     }
-  };
-  auto multiply = [&](int s, int t) {
-    const int by = 8 * (t & 3);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      intx8 b;
-      unsigned power;
-      if constexpr (RAW) {
-        b = mx6_operand(mx6_block(words[s], power));
-      } else {
-        b = intx8{(int)x4[s][i].x, (int)x4[s][i].y, (int)x4[s][i].z, (int)x4[s][i].w, (int)x2[s][i].x, (int)x2[s][i].y, 0, 0};
-        power = xp[s][i] >> by;
-      }
+      const int r = (i & 1) * 16 + r16;
 #pragma unroll
-      for (int j = 0; j < R; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(w[s][j]), b, acc[i][j], MX_FP4, MX_FP6, 0, (int)(p[s][j] >> by),
-                                                                     0, (int)power);
+      for (int q = 0; q < G; ++q) {
+        const unsigned char* tile = a_codes + ((size_t)(i >> 1) * steps + min(t0 + q, steps - 1)) * 3072;
+        x4[q][i] = *reinterpret_cast<const uint4*>(tile + g * 512 + r * 16);
+        x2[q][i] = *reinterpret_cast<const uint2*>(tile + 2048 + g * 256 + r * 8);
+      }
+      xp[i] = a_powers[((size_t)(i >> 1) * groups + (t0 >> 2)) * 128 + g * 32 + r];
     }
   };
-  const int mine = (steps - wid + NW - 1) / NW;                    // steps of this wave: wid, wid + NW, ... (none: 0)
+  load(wid);
+  for (int run = wid; run < runs; run += NW) {
+    const int t0 = run * G;
 #pragma unroll
-  for (int s = 0; s < D; ++s)
-    if (s < mine) load(s, wid + s * NW);
-  for (int base = 0; base < mine; base += D) {
+    for (int q = 0; q < G; ++q) {
+      if (q && t0 + q >= steps) break;
+      const int by = 8 * ((t0 + q) & 3);
 #pragma unroll
-    for (int s = 0; s < D; ++s)
-      if (base + s < mine) {
-        multiply(s, wid + (base + s) * NW);
-        if (base + s + D < mine) load(s, wid + (base + s + D) * NW);
+      for (int i = 0; i < MT; ++i) {
+        const intx8 b = {(int)x4[q][i].x, (int)x4[q][i].y, (int)x4[q][i].z, (int)x4[q][i].w, (int)x2[q][i].x, (int)x2[q][i].y, 0, 0};
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(w[q][j]), b, acc[i][j], MX_FP4, MX_FP6, 0, (int)(p[j] >> by), 0,
+                                                                       (int)(xp[i] >> by));
       }
+    }
+    load(run + NW);                                                // (past the end: the last place again)
+    __builtin_amdgcn_sched_barrier(0);
   }
-  // D[n][m]: m = lane % 16, n = 4 (lane / 16) + r
+#pragma unroll
   for (int i = 0; i < MT; ++i) {
     if (i) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      floatx4 v = acc[0][j];
-#pragma unroll
-      for (int q = 1; q < MT; ++q)
-        if (i == q) v = acc[q][j];
-      *reinterpret_cast<floatx4*>(&red[wid][r16][j * 16 + 4 * g]) = v;
-    }
-    __syncthreads();
-    constexpr int OUT = PAIR ? COLS / 2 : COLS;
-    for (int e = threadIdx.x; e < 16 * OUT; e += NW * 64) {
-      const int m = i * 16 + e / OUT, c = e % OUT;
-      if (m >= M) break;
-      if constexpr (PAIR) {
-        const int f = tile0 * 8 + c, at = (c >> 4) * 32 + (c & 15);
-        float gate = 0.f, up = 0.f;
-#pragma unroll
-        for (int q = 0; q < NW; ++q) {
-          gate += red[q][e / OUT][at];
-          up += red[q][e / OUT][at + 16];
-        }
-        if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)gate_mul(gate, up, limit);
-      } else {
-        const int n = tile0 * 16 + c;
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < NW; ++q) v += red[q][e / OUT][c];
-        if (n < N) store_one(C, (size_t)m * N + n, bias ? v + bias[n] : v, epi);
-      }
-    }
+    few_results<R, NW, PAIR>(acc[i], red, C, bias, 16 * i, M, N, blockIdx.x * R, wid, epi, limit);
   }
 }
 
@@ -509,12 +533,22 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
 }
 
 // ------------------------------------------------------------------ which kernel
-// form: 0 `few_kernel` on rows as they come, 1 on rows in E2M3, 2 .. `tile_kernel` of TILE_FORMS[form - 2]; parts of K, groups of 512 k in each
+// form: 0 `few_kernel`, 1 `few_six_kernel`, 2 .. `tile_kernel` of TILE_FORMS[form - 2]; parts of K, groups of 512 k in each
 enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 3 };
 struct Plan { int form, splits, groups; };
 
-static Plan make_plan(int M, int w16, int groups, int n_cu) {
-  if (M <= 16) return Plan{FEW_RAW, 1, groups};
+// `whole`: rows of x whose 16-byte pieces begin at multiples of 16 bytes (as they come, `few_kernel` reads no others).
+// At most 16 rows, as they come or in E2M3 by a launch of their own in front: that launch costs some 2 us, quantising on the way as much as the
+// runs of a CU are many; what a run costs goes by how many rows share its lanes.  Microseconds, matrices from memory, as they come / in E2M3, by
+// U, the steps of a CU.  4 rows (any U): 4.1 / 6.2 (8,192 x 2,048, U 32), 12.5 / 12.9 (3,584 x 18,944, 148), 17.0 / 19.1 (37,888 x 3,584, 130).
+// 8 rows: 4.6 / 5.7 (3,584 x 3,584, 28), 9.0 / 8.6 (2,048 x 11,008, 86), 14.9 / 13.1 (148), 20.0 / 17.7 (130).  16 rows, from L2: 4.8 / 5.7
+// (2,048 x 2,048, 16), 6.3 / 6.3 (28), 11.3 / 7.7 (2,048 x 8,192, 64).
+static Plan make_plan(int M, int w16, int steps, bool whole, int n_cu) {
+  const int groups = (steps + 3) / 4;
+  if (M <= 16) {
+    const long blocks = w16 > n_cu ? (w16 + 1) / 2 : w16, u = (blocks + n_cu - 1) / n_cu * steps;
+    return Plan{whole && (M <= 4 || u <= (M <= 8 ? 80 : 24)) ? FEW_RAW : FEW_SIX, 1, groups};
+  }
   if (M <= 64) return Plan{FEW_SIX, 1, groups};
   constexpr int tile_m[N_TILE_FORMS] = {256, 256, 128}, tile_n[N_TILE_FORMS] = {256, 128, 128};
   Plan best{TILES, 1, groups};
@@ -537,11 +571,11 @@ static Plan make_plan(int M, int w16, int groups, int n_cu) {
 }
 
 // out: form, parts of K, bytes of scratch for the rows in E2M3, floats of scratch for the parts (64 bits each)
-MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int n_cu, long long* out) {
+MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int whole, int n_cu, long long* out) {
   if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
   const long long w16 = (swiglu ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
   if (w16 * 16 > (1LL << 30)) return (int)hipErrorInvalidValue;
-  const Plan p = make_plan(M, (int)w16, (int)groups, n_cu);
+  const Plan p = make_plan(M, (int)w16, (int)steps, whole, n_cu);
   out[0] = p.form;
   out[1] = p.splits;
   out[2] = p.form == FEW_RAW ? 0 : m32 * (steps * 3072 + groups * 512);
@@ -562,16 +596,13 @@ static int launch_tiles(const unsigned char* six, const void* codes, const void*
   return mf_launch_status();
 }
 
-template <typename XT, bool VEC, int MT, int D>
-static int launch_few(const XT* x, const Rows6& six, const void* codes, const void* powers, const float* bias, void* C, int M, int N, int K, int w16,
-                      int steps, int groups, int epi, float limit, hipStream_t stream) {
-  if (epi == EPI_SWIGLU)
-    few_kernel<XT, VEC, MT, 2, 8, D, true><<<(w16 + 1) / 2, 512, 0, stream>>>(x, six, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K,
-                                                                            w16, steps, groups, epi, limit);
-  else
-    few_kernel<XT, VEC, MT, 1, 8, D, false><<<w16, 512, 0, stream>>>(x, six, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K, w16,
-                                                                     steps, groups, epi, limit);
-  return mf_launch_status();
+// R, the tiles of a workgroup: gate and up, or one where every CU gets at most one so, else two
+template <typename F>
+static int with_tiles(int epi, int w16, int n_cu, F run) {
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (epi == EPI_SWIGLU) return run(Two{}, std::true_type{});
+  return w16 > n_cu ? run(Two{}, std::false_type{}) : run(One{}, std::false_type{});
 }
 
 // C [M][N] (float32, added to where epi is EPI_ACC_F32, or bfloat16) from x [M][K] (bfloat16 or float32) and the stored [N][K]; EPI_SWIGLU: C is
@@ -579,39 +610,50 @@ static int launch_few(const XT* x, const Rows6& six, const void* codes, const vo
 MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const void* powers, const float* bias, void* C, void* scratch, float* part,
                          int M, int N, int K, int epi, float limit, int n_cu, hipStream_t stream) {
   long long sizes[4];
-  const int bad = mf_mx4_plan(M, N, K, epi == EPI_SWIGLU, n_cu, sizes);
+  const bool vec = (uintptr_t)x % 16 == 0 && K % (is_bf16 ? 8 : 4) == 0;
+  const int bad = mf_mx4_plan(M, N, K, epi == EPI_SWIGLU, vec, n_cu, sizes);
   if (bad) return bad;
   const int w16 = (epi == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  const Plan p = make_plan(M, w16, groups, n_cu);
-  const bool vec = (uintptr_t)x % 16 == 0 && K % (is_bf16 ? 8 : 4) == 0;
-  Rows6 six{(const unsigned char*)scratch, (const unsigned*)((const unsigned char*)scratch + (size_t)m32 * steps * 3072)};
-  if (p.form == FEW_RAW) {
-    auto run = [&](auto T0, auto VEC) {
-      using T = decltype(T0);
-      return launch_few<T, decltype(VEC)::value, 1, sizeof(T) == 2 ? 4 : 2>((const T*)x, six, codes, powers, bias, C, M, N, K, w16, steps, groups,
-                                                                          epi, limit, stream);
-    };
-    if (is_bf16) return vec ? run(bf16{}, std::true_type{}) : run(bf16{}, std::false_type{});
-    return vec ? run(float{}, std::true_type{}) : run(float{}, std::false_type{});
-  }
+  const Plan p = make_plan(M, w16, steps, vec, n_cu);
+  unsigned* a_powers = (unsigned*)((unsigned char*)scratch + (size_t)m32 * steps * 3072);
+  if (p.form == FEW_RAW)
+    return with_tiles(epi, w16, n_cu, [&](auto R0, auto PAIR) {
+      constexpr int R = decltype(R0)::value;
+      auto run = [&](auto T0, auto G0) {
+        using T = decltype(T0);
+        constexpr int G = decltype(G0)::value;
+        few_kernel<T, R, 8, G == 1 ? 2 : 1, G, decltype(PAIR)::value><<<(w16 + R - 1) / R, 512, 0, stream>>>(
+            (const T*)x, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, K, w16, steps, groups, epi, limit);
+        return mf_launch_status();
+      };
+      auto typed = [&](auto G) { return is_bf16 ? run(bf16{}, G) : run(float{}, G); };
+      if (M <= 4) return typed(std::integral_constant<int, 4>{});
+      if (M <= 8) return typed(std::integral_constant<int, 2>{});
+      return typed(std::integral_constant<int, 1>{});
+    });
   if (!scratch || (p.splits > 1 && !part)) return (int)hipErrorInvalidValue;
   auto quantise = [&](auto T0, auto VEC) {
     using T = decltype(T0);
     const size_t units = (size_t)m32 * 8 * groups;
-    rows_kernel<T, decltype(VEC)::value><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>((const T*)x, (unsigned char*)scratch, (unsigned*)six.powers, M,
+    rows_kernel<T, decltype(VEC)::value><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>((const T*)x, (unsigned char*)scratch, a_powers, M,
                                                                                         m32, K, steps, groups);
   };
   if (is_bf16) vec ? quantise(bf16{}, std::true_type{}) : quantise(bf16{}, std::false_type{});
   else vec ? quantise(float{}, std::true_type{}) : quantise(float{}, std::false_type{});
   int rc = mf_launch_status();
   if (rc) return rc;
-  if (p.form == FEW_SIX) {
-    auto run = [&](auto MT) {
-      return launch_few<void, true, decltype(MT)::value, 4>((const void*)nullptr, six, codes, powers, bias, C, M, N, K, w16, steps, groups, epi, limit, stream);
-    };
-    if (M <= 32) return run(std::integral_constant<int, 2>{});
-    return run(std::integral_constant<int, 4>{});
-  }
+  if (p.form == FEW_SIX)
+    return with_tiles(epi, w16, n_cu, [&](auto R0, auto PAIR) {
+      constexpr int R = decltype(R0)::value;
+      auto run = [&](auto MT) {
+        few_six_kernel<decltype(MT)::value, R, 8, 2, decltype(PAIR)::value><<<(w16 + R - 1) / R, 512, 0, stream>>>(
+            (const unsigned char*)scratch, a_powers, (const uint4*)codes, (const unsigned*)powers, bias, C, M, N, w16, steps, groups, epi, limit);
+        return mf_launch_status();
+      };
+      if (M <= 16) return run(std::integral_constant<int, 1>{});
+      if (M <= 32) return run(std::integral_constant<int, 2>{});
+      return run(std::integral_constant<int, 4>{});
+    });
   auto tiles = [&](auto BM, auto BN, auto STAGES, auto PER_CU, auto PAIR) {
     return launch_tiles<decltype(BM)::value, decltype(BN)::value, decltype(STAGES)::value, decltype(PER_CU)::value, decltype(PAIR)::value>((const unsigned char*)scratch, codes, powers, bias, C, part, M, N,
                                                                                      m32, w16, steps, groups, p, epi, limit, stream);

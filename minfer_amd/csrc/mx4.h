@@ -19,6 +19,8 @@
 // Rows in 6 bits (scratch of a product), `[m][k]`: per 32 rows and 128 k three kilobytes: [4 g][32 r][16 bytes], the first 21 values and a third
 // of one, then [4 g][32 r][8 bytes]; powers [ceil(m / 32)][ceil(k / 512)][4 g][32 r][4 bytes].
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 typedef int intx8 __attribute__((ext_vector_type(8)));
@@ -66,7 +68,12 @@ __device__ __forceinline__ uintx6 mx6_block(const unsigned (&words)[32], unsigne
     even[i] = __uint_as_float(words[2 * i]);
     odd[i] = __uint_as_float(words[2 * i + 1]);
   }
-  return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, mx_unit(power));
+  // (The compiler may give this instruction's result registers of its operands, and it reads its divisor again after its first results: with
+  // the divisor's register among them every block came out wrong.  Hence in assembly, whose result shares none; behind it the wait that the
+  // compiler sets behind a conversion of this kind.)
+  uintx6 six;
+  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 1" : "=&v"(six) : "v"(even), "v"(odd), "v"(mx_unit(power)));
+  return six;
 }
 
 __device__ __forceinline__ intx8 mx6_operand(const uintx6& c) {
@@ -74,25 +81,119 @@ __device__ __forceinline__ intx8 mx6_operand(const uintx6& c) {
 }
 __device__ __forceinline__ intx8 mx4_operand(const uint4& c) { return intx8{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0}; }
 
-// The words of the block of 32 values of a row that begins at value k0, zeros from k_end on.  VEC: rows and k_end allow 16-byte loads of whole ones.
-template <bool VEC, int W, typename T>
-__device__ __forceinline__ void mx_load_block(const T* __restrict__ row, int k0, int k_end, unsigned (&words)[W]) {
-  constexpr int PER = 16 / sizeof(T);              // values of a 16-byte load
+// The words of the block of 32 values of a row that begins at value k0, zeros from k_end on, in loads of 16 bytes: the row and k_end allow them.
+template <int W, typename T>
+__device__ __forceinline__ void mx_load_block(const T* row, int k0, int k_end, unsigned (&words)[W]) {
+  constexpr int PER = 16 / sizeof(T);              // values of a load
 #pragma unroll
   for (int i = 0; i < 32 / PER; ++i) {
-    uint4 v = uint4{0, 0, 0, 0};
-    const int k = k0 + i * PER;
-    if (VEC) {
-      if (k < k_end) v = *reinterpret_cast<const uint4*>(row + k);
-    } else {
-      alignas(16) T raw[PER];
-#pragma unroll
-      for (int j = 0; j < PER; ++j) raw[j] = k + j < k_end ? row[k + j] : (T)0.f;
-      v = *reinterpret_cast<const uint4*>(raw);
-    }
+    const uint4 v = k0 + i * PER < k_end ? *reinterpret_cast<const uint4*>(row + k0 + i * PER) : uint4{0, 0, 0, 0};
     words[4 * i] = v.x;
     words[4 * i + 1] = v.y;
     words[4 * i + 2] = v.z;
     words[4 * i + 3] = v.w;
   }
+}
+
+// Values k0 .. k0 + 511 of four rows [..][k] from row0 on into LDS, zeros past row m and past k, by one wave: for rows that begin anywhere.
+template <typename T, int PITCH>
+__device__ __forceinline__ void mx_stage_rows(const T* __restrict__ x, T (*stage)[PITCH], int row0, int m, int k, int k0, int lane) {
+  T v[4][8];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = k0 + i * 64 + lane;
+      v[r][i] = row0 + r < m && at < k ? x[(size_t)(row0 + r) * k + at] : (T)0.f;
+    }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) stage[r][i * 64 + lane] = v[r][i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// lane i of 16 gets lane (i + BY) % 16's
+template <int BY>
+__device__ __forceinline__ unsigned rotate_down(unsigned v) {
+  if constexpr (BY == 0) return v;
+  else return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + 16 - BY, 0xf, 0xf, false);      // (row_ror)
+}
+
+// A run of G steps of 128 k of at most 16 / G rows of x as they come, against R tiles of 16 matrix rows: what a lane asks for, and the run's products
+// (16x16x128: A = 16 matrix rows as they are stored, B = rows of x, a lane holding one block of one row, so that quantising it takes no other
+// lane).  At most 8 (4) rows fill half (a quarter) of the lanes: with G of 2 (4) the others take the same rows' blocks of the next step (the
+// next three), one quantising serves the run, and its later steps get their operands by a rotation within 16 lanes (what the columns past
+// the rows then hold, nobody reads).  Lane: g = lane / 16, sub = lane % 16 / (16 / G) the step of the run that it takes.
+template <typename XT, int R, int G>
+struct FewRun {
+  static constexpr int W = sizeof(XT) * 8, PER = 16 / sizeof(XT), ROWS = 16 / G;
+  static_assert(G == 1 || G == 2 || G == 4, "a run's powers lie in one word");
+  uint4 w[G][R];
+  unsigned p[R], words[W];
+  // row: the lane's, its 16-byte pieces at multiples of 16 bytes; wtile, wpow: the tiles' first places of this lane; t0: the run's first step
+  __device__ __forceinline__ void load(const XT* row, const uint4* const (&wtile)[R], const unsigned* const (&wpow)[R], int t0, int sub, int g,
+                                       int steps, int K) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+#pragma unroll
+      for (int q = 0; q < G; ++q) w[q][j] = wtile[j][(size_t)min(t0 + q, steps - 1) * 64];
+      p[j] = wpow[j][(size_t)(t0 >> 2) * 64];
+    }
+#pragma unroll
+    for (int q = 0; q < W / 4; ++q) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + min((t0 + sub) * 128 + g * 32 + q * PER, K - PER));
+      words[4 * q] = v.x, words[4 * q + 1] = v.y, words[4 * q + 2] = v.z, words[4 * q + 3] = v.w;
+    }
+  }
+  // acc[n][m]: m = lane % 16, n = 4 (lane / 16) + r
+  __device__ __forceinline__ void multiply(floatx4 (&acc)[R], int t0, int sub, int g, int steps, int K) {
+    if ((t0 + G) * 128 > K) {                                      // what was asked for past the row's end
+#pragma unroll
+      for (int q = 0; q < W; ++q) words[q] = (t0 + sub) * 128 + g * 32 + q / 4 * PER < K ? words[q] : 0;
+    }
+    unsigned power;
+    const uintx6 block = mx6_block(words, power);
+    auto one = [&](auto Q) {
+      constexpr int q = decltype(Q)::value;
+      if (q && t0 + q >= steps) return;
+      intx8 b = {};
+#pragma unroll
+      for (int z = 0; z < 6; ++z) b[z] = (int)rotate_down<q * ROWS>(block[z]);
+      const int by = 8 * ((t0 + q) & 3), with = (int)rotate_down<q * ROWS>(power);
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(w[q][j]), b, acc[j], MX_FP4, MX_FP6, 0, (int)(p[j] >> by), 0, with);
+    };
+    one(std::integral_constant<int, 0>{});
+    if constexpr (G > 1) one(std::integral_constant<int, 1>{});
+    if constexpr (G > 2) {
+      one(std::integral_constant<int, 2>{});
+      one(std::integral_constant<int, 3>{});
+    }
+  }
+};
+
+// A wave's share of R tiles over the whole of K: the runs wid, wid + NW, .., D of them in flight.  No load stands behind a condition (there the
+// compiler would wait for all that are in flight): past the end they ask for the last place again.
+template <typename XT, int R, int NW, int D, int G>
+__device__ __forceinline__ void few_rows(const XT* row, const uint4* const (&wtile)[R], const unsigned* const (&wpow)[R], int wid, int sub, int g,
+                                         int steps, int K, floatx4 (&acc)[R]) {
+  const int runs = (steps + G - 1) / G, mine = (runs - wid + NW - 1) / NW, last = max(mine, 1) - 1, first = min(wid, runs - 1);
+  FewRun<XT, R, G> run[D];
+#pragma unroll
+  for (int s = 0; s < D; ++s) run[s].load(row, wtile, wpow, (first + min(s, last) * NW) * G, sub, g, steps, K);
+  int base = 0;
+  for (; base + D < mine; base += D) {
+#pragma unroll
+    for (int s = 0; s < D; ++s) {
+      run[s].multiply(acc, (first + (base + s) * NW) * G, sub, g, steps, K);
+      run[s].load(row, wtile, wpow, (first + min(base + s + D, last) * NW) * G, sub, g, steps, K);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < D; ++s)
+    if (base + s < mine) run[s].multiply(acc, (first + (base + s) * NW) * G, sub, g, steps, K);
 }

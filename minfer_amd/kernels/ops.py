@@ -162,12 +162,12 @@ _PROTOTYPES = {
         "mf_mx4_dequantise": [_P, _P, _P, c_int, c_int, c_int, _P],
     },
     "gemm_mx4": {
-        "mf_mx4_plan": [c_int, c_int, c_int, c_int, c_int, _P],
+        "mf_mx4_plan": [c_int, c_int, c_int, c_int, c_int, c_int, _P],
         "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, c_int, _P],
     },
     "moe_mx4": {
-        "mf_mx4_moe": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
-                       c_int, _P],
+        "mf_mx4_moe": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                       c_int, c_int, c_int, _P],
     },
     "attn_tokens_f32": {
         "mf_attn_tokens_f32": [_P, _P, _P, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
@@ -1548,8 +1548,10 @@ def mx4_moe_sparse(x: torch.Tensor, gate_up: torch.Tensor, gate_up_powers: torch
                           f"{MOE_SPARSE_PAIRS} pairs and {MOE_MAX_EXPERTS} experts")
     _aligned("mx4_moe_sparse", gate_up=gate_up, gate_up_powers=gate_up_powers, down=down, down_powers=down_powers)
     y = torch.empty((n_tok * top, 16 * tiles), dtype=torch.bfloat16, device=x.device)
-    _check(_fn("moe_mx4", "mf_mx4_moe")(x, _is_bf16(x), gate_up, gate_up_powers, down, down_powers, chosen, weights, y, out, _is_bf16(out), n_tok,
-                                        top, E, ff, K, N, float(limit), int(act), 1 if accumulate else 0, 1 if hands_on else 0, _stream()),
+    rows = None if _whole(x) else torch.empty((n_tok, (K + 15) // 16 * 16), dtype=x.dtype, device=x.device)
+    _check(_fn("moe_mx4", "mf_mx4_moe")(x, _is_bf16(x), gate_up, gate_up_powers, down, down_powers, chosen, weights, y, rows, out, _is_bf16(out),
+                                        n_tok, top, E, ff, K, N, float(limit), int(act), 1 if accumulate else 0, 1 if hands_on else 0,
+                                        cu_count(), _stream()),
            "mx4_moe_sparse")
 
 
@@ -2247,10 +2249,16 @@ def _aligned(what: str, **tensors: torch.Tensor) -> None:
             raise KernelError(f"{what}.{name}: must begin at a multiple of 16 bytes")
 
 
+def _whole(x: torch.Tensor) -> bool:
+    """Whether every row of x begins at a multiple of 16 bytes."""
+    return not (x.data_ptr() % 16 or x.shape[1] % (8 if x.dtype == torch.bfloat16 else 4))
+
+
 @functools.lru_cache(maxsize=4096)
-def _mx4_plan(m: int, n: int, k: int, swiglu: bool, n_cu: int) -> Tuple[int, int, int, int]:
+def _mx4_plan(m: int, n: int, k: int, swiglu: bool, whole: bool, n_cu: int) -> Tuple[int, int, int, int]:
+    """(kernel, parts of K, bytes of scratch for the rows, floats of scratch for the parts); `whole`: x allows 16-byte loads."""
     out = (c_int64 * 4)()
-    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, 1 if swiglu else 0, n_cu, out)
+    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, 1 if swiglu else 0, 1 if whole else 0, n_cu, out)
     if rc != 0:
         raise KernelError(f"mx4_linear: error {rc} for m {m}, n {n}, k {k}")
     return tuple(out)
@@ -2264,7 +2272,7 @@ def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.
         return
     _aligned(what, codes=codes, powers=powers)
     n_cu = cu_count()
-    _, _, six, parts = _mx4_plan(m, n, k, epi == EPI_SWIGLU, n_cu)
+    _, _, six, parts = _mx4_plan(m, n, k, epi == EPI_SWIGLU, _whole(x), n_cu)
     scratch = torch.empty(six, dtype=torch.uint8, device=x.device) if six else None
     part = torch.empty(parts, dtype=torch.float32, device=x.device) if parts else None
     _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, limit, n_cu, _stream()),

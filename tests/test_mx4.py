@@ -40,13 +40,14 @@ def test_host_tensors_are_refused():
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (896, 896), (3584, 18944), (4608, 3584), (152064, 3584), (100, 40000)])
 def test_every_plan_covers_its_product(m, n, k):
     """The parts of K of a plan cover it, none of them is empty, and the scratch is that of its kernels."""
-    for swiglu in (False, True):
-        form, splits, six, parts = ops._mx4_plan(m, n, k, swiglu, 256)
+    for swiglu, whole in ((False, True), (True, True), (False, False), (True, False)):
+        form, splits, six, parts = ops._mx4_plan(m, n, k, swiglu, whole, 256)
         groups, steps, w16 = -(-k // 512), -(-k // 128), -(-n // 16) * (2 if swiglu else 1)
         per = -(-groups // splits)
         assert 1 <= splits <= groups and (splits - 1) * per < groups <= splits * per
         assert parts == (splits * m * w16 * 16 if splits > 1 else 0)
-        assert six == (0 if m <= 16 else -(-m // 32) * (steps * 3072 + groups * 512))
+        assert m <= 16 and whole or form > 0
+        assert six == (0 if form == 0 else -(-m // 32) * (steps * 3072 + groups * 512))
 
 
 def test_weights_option():

@@ -296,6 +296,27 @@ def test_experts_odd_choices():
     assert (out[1] == 0).all()
 
 
+@pytest.mark.parametrize("tokens", [3, 7, 12])
+def test_experts_keep_tokens_apart(tokens):
+    """A token with an infinity is NaN; the others are what they are without it, whoever shares their experts."""
+    from minfer_amd.kernels import ops
+    e, f, k = 5, 96, 160
+    layer, _ = experts(e, f, k, 8)
+    gen = torch.Generator().manual_seed(tokens)
+    chosen = torch.rand((tokens, e), generator=gen).argsort(-1)[:, :2].to(torch.int32).contiguous().to(DEV)
+    weights = torch.rand((tokens, 2), generator=gen).to(DEV)
+    x = normal((tokens, k), 4)
+    bad = x.clone()
+    bad[1, 5] = float("inf")
+    outs = []
+    for rows in (x, bad):
+        outs.append(torch.full((tokens, k), float("nan"), device=DEV))
+        ops.mx4_moe_sparse(rows, *layer, chosen, weights, outs[-1], f, act=1, accumulate=False)
+    assert torch.isnan(outs[1][1]).all() and torch.isfinite(outs[0]).all()
+    others = [t for t in range(tokens) if t != 1]
+    assert torch.equal(outs[0][others], outs[1][others])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_experts_that_hand_on(dtype):
     from minfer_amd.kernels import ops
