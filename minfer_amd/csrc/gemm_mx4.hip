@@ -28,25 +28,23 @@ __device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float
 }
 
 // ------------------------------------------------------------------ rows in E2M3
-// A lane takes a block: a wave four rows and 512 k.  Bound by memory: 2 or 4 bytes a value read, 25/32 written.  Rows that do not begin at
-// multiples of 16 bytes come by way of LDS, 64 neighbouring values a load (value by value from the row itself, 32 loads of 64 lines each: 6.2 us
-// for 37 rows of 2,500, ROWS so).
-template <typename T, bool VEC>
+// A wave takes four rows' 512 k, a lane a block of them (`MxStage`: with 64 bytes a lane straight from the rows 4,096 of 3,584 took 12.5 us, 37 of
+// 2,500, value by value, 6.2).  Bound by memory: 2 or 4 bytes a value read, 25/32 written.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned* __restrict__ powers,
-                                                   int m, int m32, int k, int steps, int groups) {
+                                                   int m, int k, int steps, int groups) {
+  __shared__ MxStage<T> stages[4];
   const int lane = threadIdx.x & 63, i = lane >> 4, c = lane & 15;
-  const size_t unit = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int four = (int)(unit / groups), group = (int)(unit - (size_t)four * groups);
+  // (a workgroup's four waves write neighbouring pieces of the same tiles: whole lines)
+  const int sixteen = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - (unsigned)sixteen * groups), four = sixteen * 4 + (threadIdx.x >> 6);
   const int row = four * 4 + i;
-  if (four * 4 >= m32 * 32) return;
+  MxStage<T>& stage = stages[threadIdx.x >> 6];
+  mx_stage_rows<WHOLE>(x, stage, four * 4, m, k, group * 512, lane);
   unsigned words[sizeof(T) * 8];
-  if constexpr (VEC) {
-    mx_load_block(x + (size_t)min(row, m - 1) * k, group * 512 + c * 32, row < m ? k : 0, words);
-  } else {
-    __shared__ __attribute__((aligned(16))) T stage[4][4][512 + 16 / sizeof(T)];
-    T (*mine)[512 + 16 / sizeof(T)] = stage[threadIdx.x >> 6];
-    mx_stage_rows(x, mine, four * 4, m, k, group * 512, lane);
-    mx_load_block(&mine[i][0], c * 32, 512, words);
+#pragma unroll
+  for (int p = 0; p < MxStage<T>::PIECES; ++p) {
+    const uint4 v = stage.at[i][MxStage<T>::place(c, p)];
+    words[4 * p] = v.x, words[4 * p + 1] = v.y, words[4 * p + 2] = v.z, words[4 * p + 3] = v.w;
   }
   unsigned power;
   const uintx6 six = mx6_block(words, power);
@@ -574,7 +572,7 @@ static Plan make_plan(int M, int w16, int steps, bool whole, int n_cu) {
 MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int whole, int n_cu, long long* out) {
   if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
   const long long w16 = (swiglu ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  if (w16 * 16 > (1LL << 30)) return (int)hipErrorInvalidValue;
+  if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30)) return (int)hipErrorInvalidValue;
   const Plan p = make_plan(M, (int)w16, (int)steps, whole, n_cu);
   out[0] = p.form;
   out[1] = p.splits;
@@ -634,9 +632,8 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
   if (!scratch || (p.splits > 1 && !part)) return (int)hipErrorInvalidValue;
   auto quantise = [&](auto T0, auto VEC) {
     using T = decltype(T0);
-    const size_t units = (size_t)m32 * 8 * groups;
-    rows_kernel<T, decltype(VEC)::value><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>((const T*)x, (unsigned char*)scratch, a_powers, M,
-                                                                                        m32, K, steps, groups);
+    rows_kernel<T, decltype(VEC)::value><<<(unsigned)(m32 * 2) * groups, 256, 0, stream>>>((const T*)x, (unsigned char*)scratch, a_powers, M, K, steps,
+                                                                                         groups);
   };
   if (is_bf16) vec ? quantise(bf16{}, std::true_type{}) : quantise(bf16{}, std::false_type{});
   else vec ? quantise(float{}, std::true_type{}) : quantise(float{}, std::false_type{});

@@ -1,11 +1,14 @@
 // The chosen experts of few tokens, their matrices in microscaled 4-bit numbers (`mx4.h`): a whole layer in two kernels, for steps of at most
 // 16 tokens and 128 (token, choice) pairs.
 //
-//   up:    y[pair][f] = act(gate_e x', up_e x') in bfloat16: a workgroup owns 16 gate rows and the 16 up rows beside them of one chosen expert.
+//   up:    y[pair][f] = act(gate_e x', up_e x') in bfloat16 and then E2M3: a workgroup owns 32 gate rows and the 32 up rows beside them of
+//          one chosen expert, which is a block of y of each of the expert's tokens.
 //   down:  out[t][n] (+)= sum over t's choices of w down_e y': a workgroup owns 16 output rows of every chosen expert, one after the other, so
 //          nothing is left to add up behind it.
 //
-// x' and y' are the rows in E2M3, made in registers on the way (`mx6_block`).  In both kernels the 16 columns of the 16x16x128 instruction are the
+// x' is the rows in E2M3, made in registers on the way (`mx6_block`); y' as the up kernel leaves it, 32 bytes a block: 24 of codes, the power
+// in the next.  (With y in bfloat16 and quantised by every workgroup of the down kernel that took 16.5 us of 8 tokens' two of 8 experts of 4,096 x
+// 2,048, DOWN so.)  In both kernels the 16 columns of the 16x16x128 instruction are the
 // step's tokens, whoever's turn it is: a token that has not chosen the expert is a column of zeros and asks for nothing.  So every chosen
 // expert's matrices are read once, whatever the number of its tokens, and the down kernel weighs what an instruction gives by the token's weight and
 // adds it up in registers.  Sums are in 32 bits in an order that the sizes and the choices fix.
@@ -43,14 +46,15 @@ __global__ __launch_bounds__(256) void whole_rows_kernel(const XT* __restrict__ 
   if (k < pitch) out[(size_t)blockIdx.y * pitch + k] = k < K ? x[(size_t)blockIdx.y * K + k] : (XT)0.f;
 }
 
-// grid (runs of R / 2 tiles of 16 f, experts or pairs): by_pair: the workgroup's expert is that of pair blockIdx.y, if no earlier pair has it
-template <typename XT, int R, int NW, int G>
+// grid (blocks of 32 f, experts or pairs): by_pair: the workgroup's expert is that of pair blockIdx.y, if no earlier pair has it
+template <typename XT, int NW, int G>
 __global__ __launch_bounds__(NW * 64) void experts_up_kernel(const XT* __restrict__ x, const uint4* __restrict__ codes,
                                                              const unsigned* __restrict__ powers, const int* __restrict__ chosen,
-                                                             bf16* __restrict__ y, int T, int top, int E, int by_pair, int K, int tiles,
+                                                             uint4* __restrict__ y, int T, int top, int E, int by_pair, int K, int tiles,
                                                              int steps, int groups, float limit, int act) {
-  constexpr int ROWS = 16 / G;
+  constexpr int ROWS = 16 / G, R = 4;
   __shared__ __attribute__((aligned(16))) float red[NW][16][16 * R + 4];
+  __shared__ __attribute__((aligned(16))) bf16 rounded[16][32 + 8];
   __shared__ int first_of[16];
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -85,26 +89,69 @@ __global__ __launch_bounds__(NW * 64) void experts_up_kernel(const XT* __restric
 #pragma unroll
   for (int j = 0; j < R; ++j) *reinterpret_cast<floatx4*>(&red[wid][r16][16 * j + 4 * g]) = acc[j];
   __syncthreads();
-  for (int i = threadIdx.x; i < 128 * R; i += NW * 64) {
-    const int to = i / (8 * R), c = i % (8 * R), at = (c >> 4) * 32 + (c & 15), f = blockIdx.x * 8 * R + c, pair = first_of[to];
-    if (pair < 0 || f >= tiles * 16) continue;
+  for (int i = threadIdx.x; i < 16 * 32; i += NW * 64) {
+    const int to = i / 32, c = i % 32, at = (c >> 4) * 32 + (c & 15);
     float gate = 0.f, up = 0.f;
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
       gate += red[q][to][at];
       up += red[q][to][at + 16];
     }
-    y[(size_t)pair * tiles * 16 + f] = (bf16)expert_gate(gate, up, limit, act);        // (past F: zeros)
+    const bool inside = (int)blockIdx.x * 2 + (c >> 4) < tiles;    // (rows past F: zeros, and act(0, 0) is 0; past the last tile: its results again)
+    rounded[to][c] = inside ? (bf16)expert_gate(gate, up, limit, act) : (bf16)0.f;
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 && first_of[threadIdx.x] >= 0) {
+    unsigned words[16], power;
+    mx_load_words(reinterpret_cast<const uint4*>(rounded[threadIdx.x]), words);
+    const uintx6 six = mx6_block(words, power);
+    uint4* to = y + ((size_t)first_of[threadIdx.x] * gridDim.x + blockIdx.x) * 2;
+    to[0] = uint4{six[0], six[1], six[2], six[3]};
+    to[1] = uint4{six[4], six[5], power, 0};
   }
 }
 
-// grid (tiles of 16 n).  y: rows of F16 values, a multiple of 16, zeros past F.  The runs of all chosen experts, one expert after the other, go to
+// A run of G steps as `FewRun`, of rows that are in E2M3 already (`blocks` blocks to a row), against one tile.
+template <int G>
+struct FewRun6 {
+  static constexpr int ROWS = 16 / G;
+  uint4 w[G], lo, hi;
+  unsigned p;
+  __device__ __forceinline__ void load(const uint4* row, const uint4* wt, const unsigned* wp, int t0, int sub, int g, int steps, int blocks) {
+#pragma unroll
+    for (int q = 0; q < G; ++q) w[q] = wt[(size_t)min(t0 + q, steps - 1) * 64];
+    p = wp[(size_t)(t0 >> 2) * 64];
+    const uint4* from = row + (size_t)min((t0 + sub) * 4 + g, blocks - 1) * 2;        // (past the last block the matrix holds zeros)
+    lo = from[0];
+    hi = from[1];
+  }
+  __device__ __forceinline__ floatx4 multiply(int t0, int steps) const {
+    floatx4 z = {0.f, 0.f, 0.f, 0.f};
+    auto one = [&](auto Q) {
+      constexpr int q = decltype(Q)::value;
+      if (q && t0 + q >= steps) return;
+      const intx8 b = {(int)rotate_down<q * ROWS>(lo.x), (int)rotate_down<q * ROWS>(lo.y), (int)rotate_down<q * ROWS>(lo.z),
+                       (int)rotate_down<q * ROWS>(lo.w), (int)rotate_down<q * ROWS>(hi.x), (int)rotate_down<q * ROWS>(hi.y), 0, 0};
+      z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(w[q]), b, z, MX_FP4, MX_FP6, 0, (int)(p >> (8 * ((t0 + q) & 3))), 0,
+                                                           (int)rotate_down<q * ROWS>(hi.z));
+    };
+    one(std::integral_constant<int, 0>{});
+    if constexpr (G > 1) one(std::integral_constant<int, 1>{});
+    if constexpr (G > 2) {
+      one(std::integral_constant<int, 2>{});
+      one(std::integral_constant<int, 3>{});
+    }
+    return z;
+  }
+};
+
+// grid (tiles of 16 n).  y: a row of `blocks` blocks a pair.  The runs of all chosen experts, one expert after the other, go to
 // the waves in turn.
 template <typename XT, typename OT, int NW, int G>
-__global__ __launch_bounds__(NW * 64) void experts_down_kernel(const bf16* __restrict__ y, const uint4* __restrict__ codes,
+__global__ __launch_bounds__(NW * 64) void experts_down_kernel(const uint4* __restrict__ y, const uint4* __restrict__ codes,
                                                                const unsigned* __restrict__ powers, const int* __restrict__ chosen,
                                                                const float* __restrict__ weights, const XT* __restrict__ x,
-                                                               OT* __restrict__ out, int T, int top, int E, int F16, int N, int tiles, int steps,
+                                                               OT* __restrict__ out, int T, int top, int E, int blocks, int N, int tiles, int steps,
                                                                int groups, int add, int hands_on) {
   constexpr int D = 2, ROWS = 16 / G;
   __shared__ __attribute__((aligned(16))) float red[NW][16][20];
@@ -116,9 +163,9 @@ __global__ __launch_bounds__(NW * 64) void experts_down_kernel(const bf16* __res
   unsigned long long left0 = __ballot(p.c0 >= 0 && p.c0 < E), left1 = __ballot(p.c1 >= 0 && p.c1 < E);
   // the expert of the loads: this lane's row and weight there, its tile
   const int runs = (steps + G - 1) / G;
-  const uint4* wt[1] = {codes + (size_t)blockIdx.x * steps * 64 + lane};
-  const unsigned* wp[1] = {powers + (size_t)blockIdx.x * groups * 64 + lane};
-  const bf16* row = y;
+  const uint4* wt = codes + (size_t)blockIdx.x * steps * 64 + lane;
+  const unsigned* wp = powers + (size_t)blockIdx.x * groups * 64 + lane;
+  const uint4* row = y;
   float weight = 0.f;
   bool mine = false;
   int at = wid;                                                    // the wave's next run, counted from the end of the expert's
@@ -134,17 +181,17 @@ __global__ __launch_bounds__(NW * 64) void experts_down_kernel(const bf16* __res
       unsigned long long ours = t < T ? choices_of(m0, m1, t, top) : 0ull;
       const int first = m0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
       mine = ours != 0;
-      row = y + (size_t)(mine ? t * top + __builtin_ctzll(ours) : first) * F16;        // (who has not chosen it: some row, not added)
+      row = y + (size_t)(mine ? t * top + __builtin_ctzll(ours) : first) * blocks * 2;        // (who has not chosen it: some row, not added)
       weight = 0.f;
       for (; ours; ours &= ours - 1) weight += weights[t * top + __builtin_ctzll(ours)];       // (an expert chosen twice: both weights)
       const size_t tile = (size_t)e * tiles + blockIdx.x;
-      wt[0] = codes + tile * steps * 64 + lane;
-      wp[0] = powers + tile * groups * 64 + lane;
+      wt = codes + tile * steps * 64 + lane;
+      wp = powers + tile * groups * 64 + lane;
     }
     return true;
   };
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  FewRun<bf16, 1, G> run[D];
+  FewRun6<G> run[D];
   float share[D];
   int t0[D];
   bool have[D], adds[D];
@@ -154,14 +201,13 @@ __global__ __launch_bounds__(NW * 64) void experts_down_kernel(const bf16* __res
     t0[s] = more ? (at + runs) * G : 0;
     share[s] = weight;
     adds[s] = mine;
-    run[s].load(row, wt, wp, t0[s], sub, g, steps, F16);           // (nothing left: some place again)
+    run[s].load(row, wt, wp, t0[s], sub, g, steps, blocks);          // (nothing left: some place again)
     at += NW;
   };
   auto multiply = [&](int s) {
-    floatx4 z[1] = {floatx4{0.f, 0.f, 0.f, 0.f}};
-    run[s].multiply(z, t0[s], sub, g, steps, F16);
+    const floatx4 z = run[s].multiply(t0[s], steps);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sum[r] = adds[s] ? fmaf(share[s], z[0][r], sum[r]) : sum[r];
+    for (int r = 0; r < 4; ++r) sum[r] = adds[s] ? fmaf(share[s], z[r], sum[r]) : sum[r];
   };
 #pragma unroll
   for (int s = 0; s < D; ++s) load(s);
@@ -192,11 +238,11 @@ __global__ __launch_bounds__(NW * 64) void experts_down_kernel(const bf16* __res
 }
 
 // x [T][K] (bfloat16 or float32); gate_up: the stored [E][2 tiles of 16][K], gate and up tiles in turn; down: the stored [E][N][F]; chosen, weights
-// [T][top]; y: scratch of T top ceil16(F) bfloat16; rows: scratch of T ceil16(K) of x's type where x or K is not a multiple of 16 bytes; out [T][N]
+// [T][top]; y: scratch of T top ceil(F / 32) blocks of 32 bytes; rows: scratch of T ceil16(K) of x's type where x or K is not a multiple of 16 bytes; out [T][N]
 // float32 (added to with `add`) or bfloat16.  Choices outside 0 .. E - 1 add nothing, or with hands_on (from E on, N == K) their token's x.
 MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const void* gate_up_powers, const void* down, const void* down_powers,
                       const int* chosen, const float* weights, void* y, void* rows, void* out, int out_bf16, int T, int top, int E, int F, int K,
-                      int N, float limit, int act, int add, int hands_on, int n_cu, hipStream_t stream) {
+                      int N, float limit, int act, int add, int hands_on, hipStream_t stream) {
   if (T < 1 || T > 16 || top < 1 || top > 64 || T * top > 128 || E < 1 || F < 1 || K < 1 || N < 1 || (hands_on && N != K) || (add && out_bf16))
     return (int)hipErrorInvalidValue;
   const int up_tiles = (F + 15) / 16, up_steps = (K + 127) / 128, up_groups = (K + 511) / 512;
@@ -210,11 +256,12 @@ MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const voi
     else whole_rows_kernel<float><<<grid, 256, 0, stream>>>((const float*)x, (float*)rows, K, pitch);
   }
   const int experts = by_pair ? T * top : E;
-  auto up = [&](auto T0, auto R0, auto NW0, auto G0) {
+  const int blocks = (F + 31) / 32;
+  auto up = [&](auto T0, auto NW0, auto G0) {
     using XT = decltype(T0);
-    constexpr int R = decltype(R0)::value, NW = decltype(NW0)::value, G = decltype(G0)::value;
-    experts_up_kernel<XT, R, NW, G><<<dim3((up_tiles * 2 + R - 1) / R, experts), NW * 64, 0, stream>>>(
-        (const XT*)(whole ? x : rows), (const uint4*)gate_up, (const unsigned*)gate_up_powers, chosen, (bf16*)y, T, top, E, by_pair, pitch, up_tiles,
+    constexpr int NW = decltype(NW0)::value, G = decltype(G0)::value;
+    experts_up_kernel<XT, NW, G><<<dim3(blocks, experts), NW * 64, 0, stream>>>(
+        (const XT*)(whole ? x : rows), (const uint4*)gate_up, (const unsigned*)gate_up_powers, chosen, (uint4*)y, T, top, E, by_pair, pitch, up_tiles,
         up_steps, up_groups, limit, act);
   };
   using std::integral_constant;
@@ -223,10 +270,9 @@ MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const voi
   using Four = integral_constant<int, 4>;
   using Eight = integral_constant<int, 8>;
   auto up_of = [&](auto T0) {
-    const bool wide = (long)up_tiles * experts > 4L * n_cu;
-    if (T <= 4) wide ? up(T0, Four{}, Four{}, Four{}) : up(T0, Two{}, Four{}, Four{});
-    else if (T <= 8) wide ? up(T0, Four{}, Eight{}, Two{}) : up(T0, Two{}, Eight{}, Two{});
-    else wide ? up(T0, Four{}, Eight{}, One{}) : up(T0, Two{}, Eight{}, One{});
+    if (T <= 4) up(T0, Four{}, Four{});
+    else if (T <= 8) up(T0, Eight{}, Two{});
+    else up(T0, Eight{}, One{});
   };
   if (is_bf16) up_of(bf16{});
   else up_of(float{});
@@ -236,8 +282,8 @@ MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const voi
     using XT = decltype(T0);
     using OT = decltype(O0);
     experts_down_kernel<XT, OT, 16, decltype(G0)::value><<<tiles, 1024, 0, stream>>>(
-        (const bf16*)y, (const uint4*)down, (const unsigned*)down_powers, chosen, weights, (const XT*)x, (OT*)out, T, top, E, up_tiles * 16, N, tiles,
-        steps, groups, add, hands_on);
+        (const uint4*)y, (const uint4*)down, (const unsigned*)down_powers, chosen, weights, (const XT*)x, (OT*)out, T, top, E, blocks, N, tiles, steps,
+        groups, add, hands_on);
   };
   auto behind_of = [&](auto T0, auto O0) {
     if (T <= 4) behind(T0, O0, Four{});

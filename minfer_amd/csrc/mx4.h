@@ -81,35 +81,62 @@ __device__ __forceinline__ intx8 mx6_operand(const uintx6& c) {
 }
 __device__ __forceinline__ intx8 mx4_operand(const uint4& c) { return intx8{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0}; }
 
-// The words of the block of 32 values of a row that begins at value k0, zeros from k_end on, in loads of 16 bytes: the row and k_end allow them.
-template <int W, typename T>
-__device__ __forceinline__ void mx_load_block(const T* row, int k0, int k_end, unsigned (&words)[W]) {
-  constexpr int PER = 16 / sizeof(T);              // values of a load
+// the words of a block of 32 bfloat16 values, 64 bytes
+__device__ __forceinline__ void mx_load_words(const uint4* from, unsigned (&words)[16]) {
 #pragma unroll
-  for (int i = 0; i < 32 / PER; ++i) {
-    const uint4 v = k0 + i * PER < k_end ? *reinterpret_cast<const uint4*>(row + k0 + i * PER) : uint4{0, 0, 0, 0};
-    words[4 * i] = v.x;
-    words[4 * i + 1] = v.y;
-    words[4 * i + 2] = v.z;
-    words[4 * i + 3] = v.w;
+  for (int i = 0; i < 4; ++i) {
+    const uint4 v = from[i];
+    words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
   }
 }
 
-// Values k0 .. k0 + 511 of four rows [..][k] from row0 on into LDS, zeros past row m and past k, by one wave: for rows that begin anywhere.
-template <typename T, int PITCH>
-__device__ __forceinline__ void mx_stage_rows(const T* __restrict__ x, T (*stage)[PITCH], int row0, int m, int k, int k0, int lane) {
-  T v[4][8];
+// Four rows' 512 values from k0 on, by way of LDS: asked for in the order of memory, 16 bytes a lane (WHOLE: the rows begin at multiples of 16
+// bytes) or a value a lane; zeros past row m and past k.  A block of 32 values lies there as pieces of 16 bytes in a rotated order, so that
+// eight lanes that read the same piece of eight neighbouring blocks meet in no bank.  One wave's; `mx_staged` is for the same wave.
+template <typename T>
+struct MxStage {
+  static constexpr int PIECES = 2 * sizeof(T), PER = 16 / sizeof(T);            // of a block; values of a piece
+  uint4 at[4][16 * PIECES];
+  __device__ __forceinline__ static int place(int block, int piece) {
+    return block * PIECES + ((piece + (sizeof(T) == 2 ? block >> 2 : block >> 1)) & (PIECES - 1));
+  }
+};
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void mx_stage_rows(const T* __restrict__ x, MxStage<T>& stage, int row0, int m, int k, int k0, int lane) {
+  constexpr int PIECES = MxStage<T>::PIECES, PER = MxStage<T>::PER;
+  if constexpr (WHOLE) {
+    uint4 v[4][PIECES / 4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = k0 + i * 64 + lane;
-      v[r][i] = row0 + r < m && at < k ? x[(size_t)(row0 + r) * k + at] : (T)0.f;
-    }
+      for (int i = 0; i < PIECES / 4; ++i) {
+        const int p = i * 64 + lane, from = k0 + p * PER;
+        v[r][i] = row0 + r < m && from < k ? *reinterpret_cast<const uint4*>(x + (size_t)(row0 + r) * k + from) : uint4{0, 0, 0, 0};
+      }
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) stage[r][i * 64 + lane] = v[r][i];
+      for (int i = 0; i < PIECES / 4; ++i) {
+        const int p = i * 64 + lane;
+        stage.at[r][MxStage<T>::place(p / PIECES, p % PIECES)] = v[r][i];
+      }
+  } else {
+    T v[4][8];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = k0 + i * 64 + lane;
+        v[r][i] = row0 + r < m && from < k ? x[(size_t)(row0 + r) * k + from] : (T)0.f;
+      }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int p = (i * 64 + lane) / PER;
+        reinterpret_cast<T*>(&stage.at[r][MxStage<T>::place(p / PIECES, p % PIECES)])[lane % PER] = v[r][i];
+      }
+  }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }

@@ -1,9 +1,8 @@
 // Matrices to microscaled 4-bit numbers and back (`mx4.h` says what those are and how they are stored).
 //
-// Both kernels are bound by memory: a value is read in 2 or 4 bytes and stored in 17/32, or the other way round.  A wave owns 16 rows and
-// 512 k, which is four tiles of codes (a kilobyte each) and one of powers (256 bytes): lane 16 i + c of load (s, j) takes the eight values
-// 8 c .. of tile s of row 4 j + i, so that a load takes 256 bytes (of bfloat16) of each of four rows, a block lies in four neighbouring lanes,
-// which find its largest magnitude by two exchanges, and a lane ends with a word of codes.
+// Both kernels are bound by memory: a value is read in 2 or 4 bytes and stored in 17/32, or the other way round.  A wave owns four rows of a
+// tile and 512 k: four neighbouring lanes hold a block, eight values each, find its largest magnitude by two exchanges and end with a word of
+// codes each; a row's sixteen blocks are sixteen pieces of 16 bytes in four tiles, and their powers 16 words of four.
 #include "mx4.h"
 
 // the largest of four neighbouring lanes
@@ -12,20 +11,9 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
   return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));     // (lanes 2 3 0 1)
 }
 
-template <typename T> struct Eight;
-template <> struct Eight<bf16> {
+// eight values of a lane
+struct Eight16 {
   uint4 v;
-  template <bool VEC>
-  __device__ __forceinline__ void load(const bf16* __restrict__ row, int k, int k_end) {
-    if (VEC) {
-      v = k < k_end ? *reinterpret_cast<const uint4*>(row + k) : uint4{0, 0, 0, 0};
-    } else {
-      alignas(16) bf16 raw[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = k + i < k_end ? row[k + i] : (bf16)0.f;
-      v = *reinterpret_cast<const uint4*>(raw);
-    }
-  }
   __device__ __forceinline__ unsigned largest() const {
     const unsigned m = max_pairs(max_pairs(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), max_pairs(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
     return max(m & 0xFFFF0000u, m << 16);
@@ -38,21 +26,8 @@ template <> struct Eight<bf16> {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v.w), unit, 3);
   }
 };
-template <> struct Eight<float> {
+struct Eight32 {
   float4 lo, hi;
-  template <bool VEC>
-  __device__ __forceinline__ void load(const float* __restrict__ row, int k, int k_end) {
-    if (VEC) {
-      lo = k < k_end ? *reinterpret_cast<const float4*>(row + k) : float4{0.f, 0.f, 0.f, 0.f};
-      hi = k + 4 < k_end ? *reinterpret_cast<const float4*>(row + k + 4) : float4{0.f, 0.f, 0.f, 0.f};
-    } else {
-      alignas(16) float raw[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = k + i < k_end ? row[k + i] : 0.f;
-      lo = *reinterpret_cast<const float4*>(raw);
-      hi = *reinterpret_cast<const float4*>(raw + 4);
-    }
-  }
   __device__ __forceinline__ unsigned largest() const {
     const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     unsigned m = 0;
@@ -69,106 +44,106 @@ template <> struct Eight<float> {
   }
 };
 
-template <typename T, bool VEC>
+// WHOLE: rows that begin at multiples of 16 bytes; others come by way of LDS.  Lane 16 i + c of step s takes the values 8 c .. of the step's 128 of row i.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx4_quantise_kernel(const T* __restrict__ w, unsigned* __restrict__ codes, unsigned* __restrict__ powers,
-                                                           int rows, int k, int tiles, int steps, int groups) {
+                                                           int rows, int k, int steps, int groups) {
+  using Eight = typename std::conditional<sizeof(T) == 2, Eight16, Eight32>::type;
   const int lane = threadIdx.x & 63;
-  const size_t unit = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int tile = (int)(unit / groups), group = (int)(unit - (size_t)tile * groups);
-  if (tile >= tiles) return;
-  const int i = lane >> 4, c = lane & 15;
-  Eight<T> v[4][4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = tile * 16 + 4 * j + i;
-      v[s][j].template load<VEC>(w + (size_t)min(row, rows - 1) * k, group * 512 + s * 128 + c * 8, row < rows ? k : 0);
-    }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int place = (c >> 2) * 16 + 4 * j + i;
-    unsigned power4 = 0;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const unsigned power = mx_power(quad_max(v[s][j].largest()), MX_E2M1_CARRY);
-      power4 |= power << (8 * s);
-      if (group * 4 + s < steps) {
-        const size_t at = ((size_t)tile * steps + group * 4 + s) * 256 + place * 4 + (c & 3);
-        codes[at] = power == 255 ? 0 : v[s][j].codes(mx_unit(power));
-      }
-    }
-    if ((c & 3) == 0) powers[((size_t)tile * groups + group) * 64 + place] = power4;
-  }
-}
-
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void mx4_dequantise_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ powers,
-                                                             T* __restrict__ out, int rows, int k, int tiles, int steps, int groups) {
-  const int lane = threadIdx.x & 63;
-  const size_t unit = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int tile = (int)(unit / groups), group = (int)(unit - (size_t)tile * groups);
-  if (tile >= tiles) return;
-  const int i = lane >> 4, c = lane & 15;
-  unsigned word[4][4], power4[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int place = (c >> 2) * 16 + 4 * j + i;
-    power4[j] = powers[((size_t)tile * groups + group) * 64 + place];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int step = min(group * 4 + s, steps - 1);
-      word[j][s] = codes[((size_t)tile * steps + step) * 256 + place * 4 + (c & 3)];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = tile * 16 + 4 * j + i;
-    if (row >= rows) continue;
-    T* __restrict__ to = out + (size_t)row * k;
+  // (a workgroup's four waves write the four quarters of the same tiles: whole lines)
+  const int tile = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - (unsigned)tile * groups), j = threadIdx.x >> 6;
+  const int i = lane >> 4, c = lane & 15, row = tile * 16 + 4 * j + i;
+  Eight v[4];
+  if constexpr (WHOLE) {
+    const T* from = w + (size_t)min(row, rows - 1) * k;
+    const int end = row < rows ? k : 0;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int at = group * 512 + s * 128 + c * 8;
-      if (at >= k) continue;
-      const float unit2 = mx_unit(power4[j] >> (8 * s) & 255);
-      alignas(16) T v[8];
-      auto pair = [&](auto Q) {
-        constexpr int q = decltype(Q)::value;
-        if constexpr (sizeof(T) == 2) {
-          const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word[j][s], unit2, q);
-          v[2 * q] = p[0];
-          v[2 * q + 1] = p[1];
-        } else {
-          const floatx2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[j][s], unit2, q);
-          v[2 * q] = p[0];
-          v[2 * q + 1] = p[1];
-        }
-      };
-      pair(std::integral_constant<int, 0>{});
-      pair(std::integral_constant<int, 1>{});
-      pair(std::integral_constant<int, 2>{});
-      pair(std::integral_constant<int, 3>{});
-      if (VEC) {
-        constexpr int PER = 16 / sizeof(T);
-#pragma unroll
-        for (int x = 0; x < 8 / PER; ++x)
-          if (at + x * PER < k) *reinterpret_cast<uint4*>(to + at + x * PER) = *reinterpret_cast<const uint4*>(v + x * PER);
+      if constexpr (sizeof(T) == 2) {
+        v[s].v = at < end ? *reinterpret_cast<const uint4*>(from + at) : uint4{0, 0, 0, 0};
       } else {
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if (at + x < k) to[at + x] = v[x];
+        v[s].lo = at < end ? *reinterpret_cast<const float4*>(from + at) : float4{0.f, 0.f, 0.f, 0.f};
+        v[s].hi = at + 4 < end ? *reinterpret_cast<const float4*>(from + at + 4) : float4{0.f, 0.f, 0.f, 0.f};
       }
+    }
+  } else {
+    __shared__ MxStage<T> stages[4];
+    MxStage<T>& stage = stages[threadIdx.x >> 6];
+    mx_stage_rows<false>(w, stage, tile * 16 + 4 * j, rows, k, group * 512, lane);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int block = s * 4 + (c >> 2);
+      if constexpr (sizeof(T) == 2) {
+        v[s].v = stage.at[i][MxStage<T>::place(block, c & 3)];
+      } else {
+        v[s].lo = *reinterpret_cast<const float4*>(&stage.at[i][MxStage<T>::place(block, 2 * (c & 3))]);
+        v[s].hi = *reinterpret_cast<const float4*>(&stage.at[i][MxStage<T>::place(block, 2 * (c & 3) + 1)]);
+      }
+    }
+  }
+  const int place = (c >> 2) * 16 + 4 * j + i;
+  unsigned power4 = 0;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const unsigned power = mx_power(quad_max(v[s].largest()), MX_E2M1_CARRY);
+    power4 |= power << (8 * s);
+    if (group * 4 + s < steps) codes[((size_t)tile * steps + group * 4 + s) * 256 + place * 4 + (c & 3)] = power == 255 ? 0 : v[s].codes(mx_unit(power));
+  }
+  if ((c & 3) == 0) powers[((size_t)tile * groups + group) * 64 + place] = power4;
+}
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void mx4_dequantise_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ powers,
+                                                             T* __restrict__ out, int rows, int k, int steps, int groups) {
+  const int lane = threadIdx.x & 63;
+  const int tile = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - (unsigned)tile * groups), j = threadIdx.x >> 6;
+  const int i = lane >> 4, c = lane & 15, row = tile * 16 + 4 * j + i, place = (c >> 2) * 16 + 4 * j + i;
+  const unsigned power4 = powers[((size_t)tile * groups + group) * 64 + place];
+  unsigned word[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) word[s] = codes[((size_t)tile * steps + min(group * 4 + s, steps - 1)) * 256 + place * 4 + (c & 3)];
+  if (row >= rows) return;
+  T* __restrict__ to = out + (size_t)row * k;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int at = group * 512 + s * 128 + c * 8;
+    if (at >= k) continue;
+    const float unit2 = mx_unit(power4 >> (8 * s) & 255);
+    alignas(16) T v[8];
+    auto pair = [&](auto Q) {
+      constexpr int q = decltype(Q)::value;
+      if constexpr (sizeof(T) == 2) {
+        const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word[s], unit2, q);
+        v[2 * q] = p[0], v[2 * q + 1] = p[1];
+      } else {
+        const floatx2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[s], unit2, q);
+        v[2 * q] = p[0], v[2 * q + 1] = p[1];
+      }
+    };
+    pair(std::integral_constant<int, 0>{});
+    pair(std::integral_constant<int, 1>{});
+    pair(std::integral_constant<int, 2>{});
+    pair(std::integral_constant<int, 3>{});
+    if (WHOLE) {
+      constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+      for (int x = 0; x < 8 / PER; ++x)
+        if (at + x * PER < k) *reinterpret_cast<uint4*>(to + at + x * PER) = *reinterpret_cast<const uint4*>(v + x * PER);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (at + x < k) to[at + x] = v[x];
     }
   }
 }
 
-// rows and k that the grid and the offsets of the kernels take: every wave of four to a workgroup has a tile and 512 k
-static bool mx4_sizes(int rows, int k, int& tiles, int& steps, int& groups, unsigned& grid) {
+// rows and k that the grid and the offsets of the kernels take: a workgroup a tile and 512 k
+static bool mx4_sizes(int rows, int k, int& steps, int& groups, unsigned& grid) {
   if (rows < 1 || k < 1 || k > (1 << 30) || rows > (1 << 30)) return false;
-  tiles = (rows + 15) / 16;
   steps = (k + 127) / 128;
   groups = (k + 511) / 512;
-  const size_t blocks = ((size_t)tiles * groups + 3) / 4;
+  const size_t blocks = (size_t)((rows + 15) / 16) * groups;
   if (blocks > 0x7FFFFFFFu) return false;
   grid = (unsigned)blocks;
   return true;
@@ -176,14 +151,13 @@ static bool mx4_sizes(int rows, int k, int& tiles, int& steps, int& groups, unsi
 
 // w [rows][k] (bfloat16, or float32) -> codes, powers
 MF_API int mf_mx4_quantise(const void* w, int is_bf16, void* codes, void* powers, int rows, int k, hipStream_t stream) {
-  int tiles, steps, groups;
+  int steps, groups;
   unsigned grid;
-  if (!mx4_sizes(rows, k, tiles, steps, groups, grid)) return (int)hipErrorInvalidValue;
+  if (!mx4_sizes(rows, k, steps, groups, grid)) return (int)hipErrorInvalidValue;
   const bool vec = (uintptr_t)w % 16 == 0 && k % (is_bf16 ? 8 : 4) == 0;
   auto run = [&](auto T0, auto VEC) {
     using T = decltype(T0);
-    mx4_quantise_kernel<T, decltype(VEC)::value><<<grid, 256, 0, stream>>>((const T*)w, (unsigned*)codes, (unsigned*)powers, rows, k, tiles,
-                                                                           steps, groups);
+    mx4_quantise_kernel<T, decltype(VEC)::value><<<grid, 256, 0, stream>>>((const T*)w, (unsigned*)codes, (unsigned*)powers, rows, k, steps, groups);
   };
   if (is_bf16) vec ? run(bf16{}, std::true_type{}) : run(bf16{}, std::false_type{});
   else vec ? run(float{}, std::true_type{}) : run(float{}, std::false_type{});
@@ -192,14 +166,14 @@ MF_API int mf_mx4_quantise(const void* w, int is_bf16, void* codes, void* powers
 
 // codes, powers -> out [rows][k] (bfloat16, or float32); exact in both, but for what is beyond the type's range
 MF_API int mf_mx4_dequantise(const void* codes, const void* powers, void* out, int is_bf16, int rows, int k, hipStream_t stream) {
-  int tiles, steps, groups;
+  int steps, groups;
   unsigned grid;
-  if (!mx4_sizes(rows, k, tiles, steps, groups, grid)) return (int)hipErrorInvalidValue;
+  if (!mx4_sizes(rows, k, steps, groups, grid)) return (int)hipErrorInvalidValue;
   const bool vec = (uintptr_t)out % 16 == 0 && k % (is_bf16 ? 8 : 4) == 0;
   auto run = [&](auto T0, auto VEC) {
     using T = decltype(T0);
     mx4_dequantise_kernel<T, decltype(VEC)::value><<<grid, 256, 0, stream>>>((const unsigned*)codes, (const unsigned*)powers, (T*)out, rows, k,
-                                                                             tiles, steps, groups);
+                                                                             steps, groups);
   };
   if (is_bf16) vec ? run(bf16{}, std::true_type{}) : run(bf16{}, std::false_type{});
   else vec ? run(float{}, std::true_type{}) : run(float{}, std::false_type{});

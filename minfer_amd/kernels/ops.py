@@ -167,7 +167,7 @@ _PROTOTYPES = {
     },
     "moe_mx4": {
         "mf_mx4_moe": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
-                       c_int, c_int, c_int, _P],
+                       c_int, c_int, _P],
     },
     "attn_tokens_f32": {
         "mf_attn_tokens_f32": [_P, _P, _P, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
@@ -1526,13 +1526,9 @@ def mx4_moe_sparse(x: torch.Tensor, gate_up: torch.Tensor, gate_up_powers: torch
         raise KernelError(f"mx4_moe_sparse: x {tuple(x.shape)}, out {tuple(out.shape)}, chosen {tuple(chosen.shape)}, gate_up {tuple(gate_up.shape)}")
     n_tok, K = x.shape
     N, E, top = out.shape[1], gate_up.shape[0], chosen.shape[1]
-    _mx4_sizes("mx4_moe_sparse", K, N, ff)
-    (tiles, *up_codes), (_, *up_powers) = mx4_shapes(ff, K)
-    down_codes, down_power = mx4_shapes(N, ff)
-    _need(gate_up, "mx4_moe_sparse.gate_up", torch.uint8, (E, 2 * tiles, *up_codes))
-    _need(gate_up_powers, "mx4_moe_sparse.gate_up_powers", torch.uint8, (E, 2 * tiles, *up_powers))
-    _need(down, "mx4_moe_sparse.down", torch.uint8, (E, *down_codes))
-    _need(down_powers, "mx4_moe_sparse.down_powers", torch.uint8, (E, *down_power))
+    up, behind = _mx4_pair_shapes(ff, K), mx4_shapes(N, ff)
+    _need_mx4("mx4_moe_sparse", gate_up, gate_up_powers, ((E, *up[0]), (E, *up[1])), "gate_up", "gate_up_powers")
+    _need_mx4("mx4_moe_sparse", down, down_powers, ((E, *behind[0]), (E, *behind[1])), "down", "down_powers")
     _need(chosen, "mx4_moe_sparse.chosen", torch.int32, (n_tok, top))
     _need(weights, "mx4_moe_sparse.weights", torch.float32, (n_tok, top))
     if accumulate and out.dtype != torch.float32:
@@ -1546,12 +1542,11 @@ def mx4_moe_sparse(x: torch.Tensor, gate_up: torch.Tensor, gate_up_powers: torch
     if not 1 <= E <= MOE_MAX_EXPERTS or not 1 <= top <= 64 or n_tok > MOE_SPARSE_TOKENS or n_tok * top > MOE_SPARSE_PAIRS:
         raise KernelError(f"mx4_moe_sparse: {n_tok} tokens with {top} of {E} experts each; it takes {MOE_SPARSE_TOKENS} tokens, "
                           f"{MOE_SPARSE_PAIRS} pairs and {MOE_MAX_EXPERTS} experts")
-    _aligned("mx4_moe_sparse", gate_up=gate_up, gate_up_powers=gate_up_powers, down=down, down_powers=down_powers)
-    y = torch.empty((n_tok * top, 16 * tiles), dtype=torch.bfloat16, device=x.device)
+    y = torch.empty((n_tok * top, (ff + 31) // 32, 32), dtype=torch.uint8, device=x.device)
     rows = None if _whole(x) else torch.empty((n_tok, (K + 15) // 16 * 16), dtype=x.dtype, device=x.device)
     _check(_fn("moe_mx4", "mf_mx4_moe")(x, _is_bf16(x), gate_up, gate_up_powers, down, down_powers, chosen, weights, y, rows, out, _is_bf16(out),
                                         n_tok, top, E, ff, K, N, float(limit), int(act), 1 if accumulate else 0, 1 if hands_on else 0,
-                                        cu_count(), _stream()),
+                                        _stream()),
            "mx4_moe_sparse")
 
 
@@ -2198,19 +2193,32 @@ def linear_gated(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, limit
 
 
 # ------------------------------------------------------------------ matrices in microscaled 4-bit numbers
+@functools.lru_cache(maxsize=4096)
 def mx4_shapes(rows: int, k: int) -> Tuple[Tuple[int, ...], Tuple[int, ...]]:
     """Shapes (both uint8) of the codes and of the powers of two that hold a matrix `[rows][k]` in microscaled 4-bit numbers
     (E2M1; 32 neighbouring values of a row share a power of two), 17/32 of a byte a value.  Codes `[ceil(rows / 16)][ceil(k / 128)][64][16]`:
     place 16 g + r of a tile holds row r's values 32 g .. 32 g + 31 of the tile's 128, two to a byte, the lower one in the low half.  Powers
     `[ceil(rows / 16)][ceil(k / 512)][64][4]`: place 16 g + r, byte s: that of row r's block 4 s + g of these 512 values, its exponent + 127
     (255: the block is NaN).  Past the rows and past k: zeros."""
+    if not (1 <= rows <= 1 << 30 and 1 <= k <= 1 << 30):
+        raise KernelError(f"microscaled matrix of sizes ({rows}, {k}) (1 to 2^30)")
     tiles = (rows + 15) // 16
     return (tiles, (k + 127) // 128, 64, 16), (tiles, (k + 511) // 512, 64, 4)
 
 
-def _mx4_sizes(what: str, *sizes: int) -> None:
-    if min(sizes) < 1 or max(sizes) > 1 << 30:
-        raise KernelError(f"{what}: sizes {sizes} (1 to 2^30)")
+@functools.lru_cache(maxsize=4096)
+def _mx4_pair_shapes(rows: int, k: int) -> Tuple[Tuple[int, ...], Tuple[int, ...]]:
+    """... of a gate and an up matrix of these sizes, tile by tile in turn (`mx4_pairs`)."""
+    (tiles, *c), (_, *p) = mx4_shapes(rows, k)
+    return (2 * tiles, *c), (2 * tiles, *p)
+
+
+def _need_mx4(what: str, codes: torch.Tensor, powers: torch.Tensor, shapes, name: str = "codes", power_name: str = "powers") -> None:
+    """Raises where a stored matrix is not of these shapes, or does not begin at a multiple of 16 bytes."""
+    _need(codes, f"{what}.{name}", torch.uint8, shapes[0])
+    _need(powers, f"{what}.{power_name}", torch.uint8, shapes[1])
+    if codes.data_ptr() % 16 or powers.data_ptr() % 16:
+        raise KernelError(f"{what}: {name} and {power_name} must begin at multiples of 16 bytes")
 
 
 def mx4_quantise(weight: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor) -> None:
@@ -2221,12 +2229,8 @@ def mx4_quantise(weight: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor
     if weight.dim() != 2:
         raise KernelError(f"mx4_quantise: weight must be a matrix, got {tuple(weight.shape)}")
     rows, k = weight.shape
-    _mx4_sizes("mx4_quantise", rows, k)
-    shapes = mx4_shapes(rows, k)
-    _need(codes, "mx4_quantise.codes", torch.uint8, shapes[0])
-    _need(powers, "mx4_quantise.powers", torch.uint8, shapes[1])
-    _aligned("mx4_quantise", codes=codes, powers=powers)
-    _check(_fn("mx4", "mf_mx4_quantise")(weight, _is_bf16(weight), codes, powers, rows, k, _stream()), f"mx4_quantise {rows}x{k}")
+    _need_mx4("mx4_quantise", codes, powers, mx4_shapes(rows, k))
+    _check(_fn("mx4", "mf_mx4_quantise")(weight, _is_bf16(weight), codes, powers, rows, k, _stream()), "mx4_quantise")
 
 
 def mx4_dequantise(codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor) -> None:
@@ -2235,18 +2239,8 @@ def mx4_dequantise(codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor)
     if out.dim() != 2:
         raise KernelError(f"mx4_dequantise: out must be a matrix, got {tuple(out.shape)}")
     rows, k = out.shape
-    _mx4_sizes("mx4_dequantise", rows, k)
-    shapes = mx4_shapes(rows, k)
-    _need(codes, "mx4_dequantise.codes", torch.uint8, shapes[0])
-    _need(powers, "mx4_dequantise.powers", torch.uint8, shapes[1])
-    _aligned("mx4_dequantise", codes=codes, powers=powers)
-    _check(_fn("mx4", "mf_mx4_dequantise")(codes, powers, out, _is_bf16(out), rows, k, _stream()), f"mx4_dequantise {rows}x{k}")
-
-
-def _aligned(what: str, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.data_ptr() % 16:
-            raise KernelError(f"{what}.{name}: must begin at a multiple of 16 bytes")
+    _need_mx4("mx4_dequantise", codes, powers, mx4_shapes(rows, k))
+    _check(_fn("mx4", "mf_mx4_dequantise")(codes, powers, out, _is_bf16(out), rows, k, _stream()), "mx4_dequantise")
 
 
 def _whole(x: torch.Tensor) -> bool:
@@ -2265,18 +2259,15 @@ def _mx4_plan(m: int, n: int, k: int, swiglu: bool, whole: bool, n_cu: int) -> T
 
 
 def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
-                 epi: int, limit: float = 0.0) -> None:
-    m, k = x.shape
-    n = out.shape[1]
+                 m: int, n: int, k: int, epi: int, limit: float) -> None:
     if m == 0:
         return
-    _aligned(what, codes=codes, powers=powers)
     n_cu = cu_count()
     _, _, six, parts = _mx4_plan(m, n, k, epi == EPI_SWIGLU, _whole(x), n_cu)
+    # (of the call's own, not shared: calls on two streams, or two graphs, do not meet in them)
     scratch = torch.empty(six, dtype=torch.uint8, device=x.device) if six else None
     part = torch.empty(parts, dtype=torch.float32, device=x.device) if parts else None
-    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, limit, n_cu, _stream()),
-           f"{what} {m}x{n}x{k}")
+    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, limit, n_cu, _stream()), what)
 
 
 def mx4_linear(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
@@ -2289,16 +2280,15 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias:
     _need(out, "mx4_linear.out", _FLOATS)
     if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0]:
         raise KernelError(f"mx4_linear: x {tuple(x.shape)}, out {tuple(out.shape)}")
-    k, n = x.shape[1], out.shape[1]
-    _mx4_sizes("mx4_linear", n, k)
-    shapes = mx4_shapes(n, k)
-    _need(codes, "mx4_linear.codes", torch.uint8, shapes[0])
-    _need(powers, "mx4_linear.powers", torch.uint8, shapes[1])
+    m, k = x.shape
+    n = out.shape[1]
+    _need_mx4("mx4_linear", codes, powers, mx4_shapes(n, k))
     if bias is not None:
         _need(bias, "mx4_linear.bias", torch.float32, (n,))
-    if accumulate and out.dtype != torch.float32:
+    half = out.dtype == torch.bfloat16
+    if accumulate and half:
         raise KernelError("mx4_linear: accumulation needs a float32 output")
-    _mx4_product("mx4_linear", x, codes, powers, bias, out, EPI_BF16 if out.dtype == torch.bfloat16 else EPI_ACC_F32 if accumulate else EPI_F32)
+    _mx4_product("mx4_linear", x, codes, powers, bias, out, m, n, k, EPI_BF16 if half else EPI_ACC_F32 if accumulate else EPI_F32, 0.0)
 
 
 def mx4_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -2312,18 +2302,14 @@ def mx4_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 def mx4_linear_swiglu(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor, limit: float = 0.0) -> None:
     """out = silu(x' G'^T) * (x' U'^T), rounded once to bfloat16, in one product; `codes`, `powers`: `mx4_pairs` of those of G and U `[f][k]`;
     x' as in `mx4_linear`, `out` bfloat16 `[m][f]`.  A `limit` above 0: the clamped form of `swiglu` with it."""
-    if limit < 0:
-        raise KernelError(f"mx4_linear_swiglu: limit {limit}")
     _need(x, "mx4_linear_swiglu.x", _FLOATS)
     _need(out, "mx4_linear_swiglu.out", torch.bfloat16)
-    if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0]:
-        raise KernelError(f"mx4_linear_swiglu: x {tuple(x.shape)}, out {tuple(out.shape)}")
-    k, f = x.shape[1], out.shape[1]
-    _mx4_sizes("mx4_linear_swiglu", 2 * f, k)
-    (tiles, *c), (_, *p) = mx4_shapes(f, k)
-    _need(codes, "mx4_linear_swiglu.codes", torch.uint8, (2 * tiles, *c))
-    _need(powers, "mx4_linear_swiglu.powers", torch.uint8, (2 * tiles, *p))
-    _mx4_product("mx4_linear_swiglu", x, codes, powers, None, out, EPI_SWIGLU, float(limit))
+    if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0] or limit < 0:
+        raise KernelError(f"mx4_linear_swiglu: x {tuple(x.shape)}, out {tuple(out.shape)}, limit {limit}")
+    m, k = x.shape
+    f = out.shape[1]
+    _need_mx4("mx4_linear_swiglu", codes, powers, _mx4_pair_shapes(f, k))
+    _mx4_product("mx4_linear_swiglu", x, codes, powers, None, out, m, f, k, EPI_SWIGLU, float(limit))
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
