@@ -227,7 +227,8 @@ struct Tile {
   static constexpr int I = BM / 64, J = BN / 64;                  // blocks of 32 x 32 results of a wave (2 x 2 waves)
   static constexpr int STAGES = STAGES_, A_ST = BM / 32 * 3072, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
   static constexpr int PA = BM / 32 * 512, PW = BN / 16 * 256, POW = PA + PW;                  // powers of 512 k
-  static constexpr int LA = BM / 32 * 3 / 4, LW = BN / 16 / 4, L = LA + LW;                    // copies of a wave and step
+  static constexpr int CA = BM / 32 * 3, CW = BN / 16;                                         // copies of a step: kilobytes
+  static constexpr int LA = (CA + 3) / 4, LW = (CW + 3) / 4, L = LA + LW;                      // ... of a wave
   static constexpr int NPA = BM / 64, NPW = BN / 64, LP = (NPA + NPW + 3) / 4;                 // copies of powers
   static constexpr int LDS = STAGES * STAGE + 2 * POW;
   static constexpr int ROW = (BN / 2 + 4) * 4;                    // bytes of a row of a wave's results on their way out (16 more: no two rows in a bank)
@@ -303,24 +304,24 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   const int wm = wid >> 1, wn = wid & 1;
   const unsigned lds0 = (unsigned)(uintptr_t)smem;
 
-  // copies: piece q of this wave is piece 4 q + wid of the step
+  // copies: piece q of this wave is piece 4 q + wid of the step (past the last: that one again, the same bytes to the same place)
   const unsigned char *ga[TT::LA], *gw[TT::LW], *gp[TT::LP];
   unsigned la[TT::LA], lw[TT::LW], lp[TT::LP], off_p[TT::LP];
   const unsigned off = lane * 16;
 #pragma unroll
   for (int q = 0; q < TT::LA; ++q) {
-    const int piece = q * 4 + wid, b = piece / 3, at = piece - b * 3;
+    const int piece = min(q * 4 + wid, TT::CA - 1), b = piece / 3, at = piece - b * 3;
     ga[q] = a_codes + (size_t)min(bm * (BM / 32) + b, m32 - 1) * steps * 3072 + at * 1024;
     la[q] = lds0 + piece * 1024;
   }
 #pragma unroll
   for (int q = 0; q < TT::LW; ++q) {
-    const int piece = q * 4 + wid;
+    const int piece = min(q * 4 + wid, TT::CW - 1);
     gw[q] = w_codes + (size_t)min(bn * (BN / 16) + piece, w16 - 1) * steps * 1024;
     lw[q] = lds0 + TT::A_ST + piece * 1024;
   }
 #pragma unroll
-  for (int q = 0; q < TT::LP; ++q) {                               // (a piece that two waves copy: the same bytes to the same place)
+  for (int q = 0; q < TT::LP; ++q) {
     const int piece = min(q * 4 + wid, TT::NPA + TT::NPW - 1);
     if (piece < TT::NPA) {
       const int b0 = min(bm * (BM / 32) + piece * 2, m32 - 1), b = min(bm * (BM / 32) + piece * 2 + half, m32 - 1);
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   using H1 = std::integral_constant<int, 1>;
   // products of a half, in front of its meeting and behind it; operand reads of a half; copies of a step that are set out behind the meeting of
   // the step three before it (the rest: in the first half of the next one)
-  constexpr int NM = I * J, BEFORE = NM / 4, BEHIND = NM - BEFORE, READS = I + J, EARLY = STAGES == 2 ? TT::L : TT::L * BEHIND / (NM + BEHIND);
+  constexpr int NM = I * J, BEFORE = NM / 4, BEHIND = NM - BEFORE, READS = I + J, EARLY = STAGES == 2 ? TT::L : (TT::L * BEHIND + NM + BEHIND - 1) / (NM + BEHIND);
 
 #pragma unroll
   for (int q = 0; q < TT::LP; ++q) copy_powers(q, g0);
@@ -532,8 +533,21 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
 
 // ------------------------------------------------------------------ which kernel
 // form: 0 `few_kernel`, 1 `few_six_kernel`, 2 .. `tile_kernel` of TILE_FORMS[form - 2]; parts of K, groups of 512 k in each
-enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 3 };
+enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 4 };
 struct Plan { int form, splits, groups; };
+
+// What a tile kernel and the sum behind it take, in microseconds: fixed, by the workgroups of the fullest CU, by their steps (one workgroup's
+// latency, or all of them by their products), by what is written.  Least squares over 1,066 products of 65 to 16,384 rows, 896 to 152,064 matrix rows
+// and K of 896 to 18,944 (7.6 % rms off); the plan that it finds least takes 0.5 % longer than the best on the average, 12 % at most.
+struct TileForm { int m, n; double step, step_each, fixed, each; };
+constexpr TileForm TILE_FORMS[N_TILE_FORMS] = {{256, 256, 0.617, 0.617, 8.2, 7.0}, {256, 128, 0.550, 0.372, 7.6, 1.8},
+                                               {128, 128, 0.245, 0.219, 7.2, 1.04}, {64, 64, 0.166, 0.108, 6.1, 0.62}};
+static double tile_cost(int f, int M, int w16, int steps, int splits, double out_bytes, int n_cu) {
+  const TileForm& t = TILE_FORMS[f];
+  const long tiles = (long)((M + t.m - 1) / t.m) * ((w16 * 16L + t.n - 1) / t.n) * splits, each = (tiles + n_cu - 1) / n_cu;
+  const double written = splits > 1 ? 2.9 + 0.97e-6 * M * w16 * 16 * splits + 0.27e-6 * out_bytes : 0.195e-6 * out_bytes;
+  return t.fixed + t.each * each + steps * std::max(t.step, t.step_each * each) + written;
+}
 
 // `whole`: rows of x whose 16-byte pieces begin at multiples of 16 bytes (as they come, `few_kernel` reads no others).
 // At most 16 rows, as they come or in E2M3 by a launch of their own in front: that launch costs some 2 us, quantising on the way as much as the
@@ -541,39 +555,39 @@ struct Plan { int form, splits, groups; };
 // U, the steps of a CU.  4 rows (any U): 4.1 / 6.2 (8,192 x 2,048, U 32), 12.5 / 12.9 (3,584 x 18,944, 148), 17.0 / 19.1 (37,888 x 3,584, 130).
 // 8 rows: 4.6 / 5.7 (3,584 x 3,584, 28), 9.0 / 8.6 (2,048 x 11,008, 86), 14.9 / 13.1 (148), 20.0 / 17.7 (130).  16 rows, from L2: 4.8 / 5.7
 // (2,048 x 2,048, 16), 6.3 / 6.3 (28), 11.3 / 7.7 (2,048 x 8,192, 64).
-static Plan make_plan(int M, int w16, int steps, bool whole, int n_cu) {
+static Plan make_plan(int M, int w16, int steps, bool whole, bool pair, double out_bytes, int n_cu) {
   const int groups = (steps + 3) / 4;
   if (M <= 16) {
     const long blocks = w16 > n_cu ? (w16 + 1) / 2 : w16, u = (blocks + n_cu - 1) / n_cu * steps;
     return Plan{whole && (M <= 4 || u <= (M <= 8 ? 80 : 24)) ? FEW_RAW : FEW_SIX, 1, groups};
   }
-  if (M <= 64) return Plan{FEW_SIX, 1, groups};
-  constexpr int tile_m[N_TILE_FORMS] = {256, 256, 128}, tile_n[N_TILE_FORMS] = {256, 128, 128};
-  Plan best{TILES, 1, groups};
-  double least = 1e30;
-  for (int f = 0; f < N_TILE_FORMS; ++f) {
-    const long tiles = (long)((M + tile_m[f] - 1) / tile_m[f]) * ((w16 * 16 + tile_n[f] - 1) / tile_n[f]);
+  // 17 to 64 rows: `few_six_kernel` by the steps of a CU's tiles (two and four tiles of rows: 6.5 + 0.054 us a step, 7.2 + 0.098; 90 products within
+  // 15 %) against the tiles: 32 rows, 3,584 x 18,944 14.7 / 17.4 us; 64 rows 22.0 / 18.2, swiglu of 37,888 x 3,584 36.9 / 20.8.
+  const int run = w16 > n_cu || pair ? 2 : 1;
+  const double few = (double)(((w16 + run - 1) / run + n_cu - 1) / n_cu) * run * steps;
+  Plan best{FEW_SIX, 1, groups};
+  double least = M > 64 ? 1e30 : M <= 32 ? 6.5 + 0.054 * few : 7.2 + 0.098 * few;
+  for (int f = 0; f < N_TILE_FORMS; ++f)
     for (int s = 1; s <= std::min(groups, 16); ++s) {
-      const int per = (groups + s - 1) / s, splits = (groups + per - 1) / per;
-      if (splits != s) continue;
-      const double rounds = (double)((tiles * splits + n_cu - 1) / n_cu);
-      const double work = f == 0 ? 4.0 : f == 1 ? 2.2 : 1.2;
-      const double cost = rounds * (per * work + 3.0) + (splits > 1 ? 8.0 + (double)M * w16 * splits / 1e5 : 0.0);
+      const int per = (groups + s - 1) / s;
+      if ((groups + per - 1) / per != s) continue;
+      const double cost = tile_cost(f, M, w16, std::min(per * 4, steps), s, out_bytes, n_cu);
       if (cost < least) {
         least = cost;
-        best = Plan{TILES + f, splits, per};
+        best = Plan{TILES + f, s, per};
       }
     }
-  }
   return best;
 }
 
+static double result_bytes(int M, int N, int epi) { return (double)M * N * (epi == EPI_SWIGLU || epi == EPI_BF16 ? 2 : 4); }
+
 // out: form, parts of K, bytes of scratch for the rows in E2M3, floats of scratch for the parts (64 bits each)
-MF_API int mf_mx4_plan(int M, int N, int K, int swiglu, int whole, int n_cu, long long* out) {
+MF_API int mf_mx4_plan(int M, int N, int K, int epi, int whole, int n_cu, long long* out) {
   if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
-  const long long w16 = (swiglu ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
+  const long long w16 = (epi == EPI_SWIGLU ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
   if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30)) return (int)hipErrorInvalidValue;
-  const Plan p = make_plan(M, (int)w16, (int)steps, whole, n_cu);
+  const Plan p = make_plan(M, (int)w16, (int)steps, whole, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
   out[0] = p.form;
   out[1] = p.splits;
   out[2] = p.form == FEW_RAW ? 0 : m32 * (steps * 3072 + groups * 512);
@@ -609,10 +623,10 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
                          int M, int N, int K, int epi, float limit, int n_cu, hipStream_t stream) {
   long long sizes[4];
   const bool vec = (uintptr_t)x % 16 == 0 && K % (is_bf16 ? 8 : 4) == 0;
-  const int bad = mf_mx4_plan(M, N, K, epi == EPI_SWIGLU, vec, n_cu, sizes);
+  const int bad = mf_mx4_plan(M, N, K, epi, vec, n_cu, sizes);
   if (bad) return bad;
   const int w16 = (epi == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  const Plan p = make_plan(M, w16, steps, vec, n_cu);
+  const Plan p = make_plan(M, w16, steps, vec, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
   unsigned* a_powers = (unsigned*)((unsigned char*)scratch + (size_t)m32 * steps * 3072);
   if (p.form == FEW_RAW)
     return with_tiles(epi, w16, n_cu, [&](auto R0, auto PAIR) {
@@ -660,7 +674,8 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
     switch (p.form) {
       case TILES: return tiles(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 3>{}, integral_constant<int, 1>{}, PAIR);
       case TILES + 1: return tiles(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, PAIR);
-      default: return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 3>{}, integral_constant<int, 2>{}, PAIR);
+      case TILES + 2: return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 3>{}, integral_constant<int, 2>{}, PAIR);
+      default: return tiles(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, PAIR);
     }
   };
   rc = epi == EPI_SWIGLU ? choose(std::true_type{}) : choose(std::false_type{});

@@ -2249,10 +2249,10 @@ def _whole(x: torch.Tensor) -> bool:
 
 
 @functools.lru_cache(maxsize=4096)
-def _mx4_plan(m: int, n: int, k: int, swiglu: bool, whole: bool, n_cu: int) -> Tuple[int, int, int, int]:
+def _mx4_plan(m: int, n: int, k: int, epi: int, whole: bool, n_cu: int) -> Tuple[int, int, int, int]:
     """(kernel, parts of K, bytes of scratch for the rows, floats of scratch for the parts); `whole`: x allows 16-byte loads."""
     out = (c_int64 * 4)()
-    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, 1 if swiglu else 0, 1 if whole else 0, n_cu, out)
+    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, epi, 1 if whole else 0, n_cu, out)
     if rc != 0:
         raise KernelError(f"mx4_linear: error {rc} for m {m}, n {n}, k {k}")
     return tuple(out)
@@ -2263,7 +2263,7 @@ def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.
     if m == 0:
         return
     n_cu = cu_count()
-    _, _, six, parts = _mx4_plan(m, n, k, epi == EPI_SWIGLU, _whole(x), n_cu)
+    _, _, six, parts = _mx4_plan(m, n, k, epi, _whole(x), n_cu)
     # (of the call's own, not shared: calls on two streams, or two graphs, do not meet in them)
     scratch = torch.empty(six, dtype=torch.uint8, device=x.device) if six else None
     part = torch.empty(parts, dtype=torch.float32, device=x.device) if parts else None

@@ -40,9 +40,9 @@ def test_host_tensors_are_refused():
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (896, 896), (3584, 18944), (4608, 3584), (152064, 3584), (100, 40000)])
 def test_every_plan_covers_its_product(m, n, k):
     """The parts of K of a plan cover it, none of them is empty, and the scratch is that of its kernels."""
-    for swiglu, whole in ((False, True), (True, True), (False, False), (True, False)):
-        form, splits, six, parts = ops._mx4_plan(m, n, k, swiglu, whole, 256)
-        groups, steps, w16 = -(-k // 512), -(-k // 128), -(-n // 16) * (2 if swiglu else 1)
+    for epi, whole in ((ops.EPI_F32, True), (ops.EPI_SWIGLU, True), (ops.EPI_BF16, False), (ops.EPI_SWIGLU, False)):
+        form, splits, six, parts = ops._mx4_plan(m, n, k, epi, whole, 256)
+        groups, steps, w16 = -(-k // 512), -(-k // 128), -(-n // 16) * (2 if epi == ops.EPI_SWIGLU else 1)
         per = -(-groups // splits)
         assert 1 <= splits <= groups and (splits - 1) * per < groups <= splits * per
         assert parts == (splits * m * w16 * 16 if splits > 1 else 0)
