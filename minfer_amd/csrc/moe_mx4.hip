@@ -84,7 +84,7 @@ __global__ __launch_bounds__(NW * 64) void experts_up_kernel(const XT* __restric
   floatx4 acc[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
-  few_rows<XT, R, NW, G == 1 ? 2 : 1, G>(x + (size_t)token * K, wtile, wpow, wid, r16 / ROWS, g, steps, K, acc);
+  few_rows<XT, R, NW, 1, G>(x + (size_t)token * K, wtile, wpow, wid, r16 / ROWS, g, steps, K, acc);
   // acc[f][t]: t = lane % 16, f = 4 (lane / 16) + r
 #pragma unroll
   for (int j = 0; j < R; ++j) *reinterpret_cast<floatx4*>(&red[wid][r16][16 * j + 4 * g]) = acc[j];
@@ -153,12 +153,16 @@ __global__ __launch_bounds__(NW * 64) void experts_down_kernel(const uint4* __re
                                                                const float* __restrict__ weights, const XT* __restrict__ x,
                                                                OT* __restrict__ out, int T, int top, int E, int blocks, int N, int tiles, int steps,
                                                                int groups, int add, int hands_on) {
-  constexpr int D = 2, ROWS = 16 / G;
+  constexpr int D = G == 4 ? 2 : 4, ROWS = 16 / G;                 // (runs of four steps: twice as much in flight a run)
   __shared__ __attribute__((aligned(16))) float red[NW][16][20];
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4, t = r16 % ROWS, sub = r16 / ROWS;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // (the weights by way of LDS: asked for where an expert begins, they would have the wave wait for all that it has in flight)
+  __shared__ float share_of[128];
+  if (threadIdx.x < 128) share_of[threadIdx.x] = (int)threadIdx.x < T * top ? weights[threadIdx.x] : 0.f;
   Pairs p;
   p.load(chosen, T * top, lane);
+  __syncthreads();
   // the pairs of experts that are still to come
   unsigned long long left0 = __ballot(p.c0 >= 0 && p.c0 < E), left1 = __ballot(p.c1 >= 0 && p.c1 < E);
   // the expert of the loads: this lane's row and weight there, its tile
@@ -183,7 +187,7 @@ __global__ __launch_bounds__(NW * 64) void experts_down_kernel(const uint4* __re
       mine = ours != 0;
       row = y + (size_t)(mine ? t * top + __builtin_ctzll(ours) : first) * blocks * 2;        // (who has not chosen it: some row, not added)
       weight = 0.f;
-      for (; ours; ours &= ours - 1) weight += weights[t * top + __builtin_ctzll(ours)];       // (an expert chosen twice: both weights)
+      for (; ours; ours &= ours - 1) weight += share_of[t * top + __builtin_ctzll(ours)];      // (an expert chosen twice: both weights)
       const size_t tile = (size_t)e * tiles + blockIdx.x;
       wt = codes + tile * steps * 64 + lane;
       wp = powers + tile * groups * 64 + lane;
@@ -257,10 +261,9 @@ MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const voi
   }
   const int experts = by_pair ? T * top : E;
   const int blocks = (F + 31) / 32;
-  auto up = [&](auto T0, auto NW0, auto G0) {
+  auto up = [&](auto T0, auto G0) {
     using XT = decltype(T0);
-    constexpr int NW = decltype(NW0)::value, G = decltype(G0)::value;
-    experts_up_kernel<XT, NW, G><<<dim3(blocks, experts), NW * 64, 0, stream>>>(
+    experts_up_kernel<XT, 4, decltype(G0)::value><<<dim3(blocks, experts), 256, 0, stream>>>(
         (const XT*)(whole ? x : rows), (const uint4*)gate_up, (const unsigned*)gate_up_powers, chosen, (uint4*)y, T, top, E, by_pair, pitch, up_tiles,
         up_steps, up_groups, limit, act);
   };
@@ -268,11 +271,11 @@ MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const voi
   using One = integral_constant<int, 1>;
   using Two = integral_constant<int, 2>;
   using Four = integral_constant<int, 4>;
-  using Eight = integral_constant<int, 8>;
+  // (four waves: with eight 8 tokens' two of 8 experts of 4,096 x 2,048 took 1 us longer, 16 tokens' two of 16 of 1,024 x 1,024 2.7)
   auto up_of = [&](auto T0) {
-    if (T <= 4) up(T0, Four{}, Four{});
-    else if (T <= 8) up(T0, Eight{}, Two{});
-    else up(T0, Eight{}, One{});
+    if (T <= 4) up(T0, Four{});
+    else if (T <= 8) up(T0, Two{});
+    else up(T0, One{});
   };
   if (is_bf16) up_of(bf16{});
   else up_of(float{});
@@ -281,7 +284,7 @@ MF_API int mf_mx4_moe(const void* x, int is_bf16, const void* gate_up, const voi
   auto behind = [&](auto T0, auto O0, auto G0) {
     using XT = decltype(T0);
     using OT = decltype(O0);
-    experts_down_kernel<XT, OT, 16, decltype(G0)::value><<<tiles, 1024, 0, stream>>>(
+    experts_down_kernel<XT, OT, 8, decltype(G0)::value><<<tiles, 512, 0, stream>>>(
         (const uint4*)y, (const uint4*)down, (const unsigned*)down_powers, chosen, weights, (const XT*)x, (OT*)out, T, top, E, blocks, N, tiles, steps,
         groups, add, hands_on);
   };
