@@ -64,34 +64,48 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
 // A workgroup owns R tiles of 16 matrix rows over the whole of K; its NW waves take the tiles' runs of G steps of 128 k in turn, so that at any
 // time they read neighbouring kilobytes, D runs of a wave in flight.  The waves' sums meet in LDS and are added in the waves' order.
 // What bounds it is the stream of the matrix; the rows come from L2 again for every workgroup.
+// What the sums of 16 rows (from row m0 on) are joined to, of this thread's result: asked for in front of the stream, not behind it.
+template <int R, int NW>
+struct Joined {
+  float b = 0.f, old = 0.f;
+  __device__ __forceinline__ Joined(const void* C, const float* bias, int m0, int M, int N, int tile0, int epi) {
+    static_assert(16 * 16 * R <= NW * 64, "a result a thread");
+    const int m = m0 + threadIdx.x / (16 * R), n = tile0 * 16 + threadIdx.x % (16 * R);
+    if (m >= M || n >= N) return;
+    if (bias) b = bias[n];
+    if (epi == EPI_ACC_F32) old = ((const float*)C)[(size_t)m * N + n];
+  }
+};
+
 // The sums of 16 rows (from row m0 on) as they lie in a wave -> results: what every kernel of few rows ends with.
 template <int R, int NW, bool PAIR>
-__device__ __forceinline__ void few_results(const floatx4 (&acc)[R], float (*red)[16][16 * R + 4], void* __restrict__ C,
-                                            const float* __restrict__ bias, int m0, int M, int N, int tile0, int wid, int epi, float limit) {
+__device__ __forceinline__ void few_results(const floatx4 (&acc)[R], float (*red)[16][16 * R + 4], void* __restrict__ C, const Joined<R, NW>& joined,
+                                            int m0, int M, int N, int tile0, int wid, int epi, float limit) {
   constexpr int COLS = 16 * R, OUT = PAIR ? COLS / 2 : COLS;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int j = 0; j < R; ++j) *reinterpret_cast<floatx4*>(&red[wid][r16][j * 16 + 4 * g]) = acc[j];
   __syncthreads();
-  for (int e = threadIdx.x; e < 16 * OUT; e += NW * 64) {
-    const int m = m0 + e / OUT, c = e % OUT;
-    if (m >= M) break;
-    if constexpr (PAIR) {
-      const int f = tile0 * 8 + c, at = (c >> 4) * 32 + (c & 15);
-      float gate = 0.f, up = 0.f;
+  const int e = threadIdx.x, row = e / OUT, c = e % OUT, m = m0 + row;
+  if (e >= 16 * OUT || m >= M) return;
+  if constexpr (PAIR) {
+    const int f = tile0 * 8 + c, at = (c >> 4) * 32 + (c & 15);
+    float gate = 0.f, up = 0.f;
 #pragma unroll
-      for (int q = 0; q < NW; ++q) {
-        gate += red[q][e / OUT][at];
-        up += red[q][e / OUT][at + 16];
-      }
-      if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)gate_mul(gate, up, limit);
-    } else {
-      const int n = tile0 * 16 + c;
-      float v = 0.f;
-#pragma unroll
-      for (int q = 0; q < NW; ++q) v += red[q][e / OUT][c];
-      if (n < N) store_one(C, (size_t)m * N + n, bias ? v + bias[n] : v, epi);
+    for (int q = 0; q < NW; ++q) {
+      gate += red[q][row][at];
+      up += red[q][row][at + 16];
     }
+    if (f < N) ((bf16*)C)[(size_t)m * N + f] = (bf16)gate_mul(gate, up, limit);
+  } else {
+    const int n = tile0 * 16 + c;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < NW; ++q) v += red[q][row][c];
+    v = v + joined.b + joined.old;
+    if (n >= N) return;
+    if (epi == EPI_BF16) ((bf16*)C)[(size_t)m * N + n] = (bf16)v;
+    else ((float*)C)[(size_t)m * N + n] = v;
   }
 }
 
@@ -121,12 +135,13 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(const XT* __restrict__ x, 
   const uint4* wtile[R];
   const unsigned* wpow[R];
   few_tiles<R>(codes, powers, blockIdx.x * R, tiles, steps, groups, lane, wtile, wpow);
+  const Joined<R, NW> joined(C, bias, 0, M, PAIR ? 0 : N, blockIdx.x * R, epi);
   floatx4 acc[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
   // (rows past M: columns that nobody reads)
   few_rows<XT, R, NW, D, G>(x + (size_t)min(r16 % ROWS, M - 1) * K, wtile, wpow, wid, r16 / ROWS, lane >> 4, steps, K, acc);
-  few_results<R, NW, PAIR>(acc, red, C, bias, 0, M, N, blockIdx.x * R, wid, epi, limit);
+  few_results<R, NW, PAIR>(acc, red, C, joined, 0, M, N, blockIdx.x * R, wid, epi, limit);
 }
 
 // At most 16 MT rows in E2M3.
@@ -193,7 +208,7 @@ __global__ __launch_bounds__(NW * 64) void few_six_kernel(const unsigned char* _
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     if (i) __syncthreads();
-    few_results<R, NW, PAIR>(acc[i], red, C, bias, 16 * i, M, N, blockIdx.x * R, wid, epi, limit);
+    few_results<R, NW, PAIR>(acc[i], red, C, Joined<R, NW>(C, bias, 16 * i, M, PAIR ? 0 : N, blockIdx.x * R, epi), 16 * i, M, N, blockIdx.x * R, wid, epi, limit);
   }
 }
 
