@@ -12,7 +12,7 @@
 enum { EPI_F32 = 0, EPI_ACC_F32 = 1, EPI_BF16 = 2, EPI_SWIGLU = 3 };
 
 // silu(g) u by the hardware's 2^x and reciprocal: off by some |g| 2^-24 of itself, far inside the rounding to bfloat16 behind it (expf and a
-// division take as long as the stores of a prompt's tile: 389 us instead of SILU for 4,096 rows of 37,888 x 3,584)
+// division take as long as the stores of a prompt's tile: 389 us instead of 350 for 4,096 rows of 37,888 x 3,584)
 __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
 }
@@ -28,8 +28,8 @@ __device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float
 }
 
 // ------------------------------------------------------------------ rows in E2M3
-// A wave takes four rows' 512 k, a lane a block of them (`MxStage`: with 64 bytes a lane straight from the rows 4,096 of 3,584 took 12.5 us, 37 of
-// 2,500, value by value, 6.2).  Bound by memory: 2 or 4 bytes a value read, 25/32 written.
+// A wave takes four rows' 512 k, a lane a block of them, by way of LDS (`MxStage`; 4,096 rows of 3,584: 10.5 us, 3.9 TB/s; straight from the rows, 64
+// bytes a lane, 12.5.  37 rows of 2,500 that begin anywhere: 3.4; value by value in a lane 6.2).  Bound by memory: 2 or 4 bytes a value read, 25/32 written.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned* __restrict__ powers,
                                                    int m, int k, int steps, int groups) {
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
   const uintx6 six = mx6_block(words, power);
   const int step = group * 4 + (c >> 2), g = c & 3, r = row & 31;
   if (step < steps) {
-    unsigned char* tile = codes + ((size_t)(row >> 5) * steps + step) * 3072;
+    unsigned char* tile = codes + ((size_t)(row >> 5) * steps + step) * MX6_TILE;
     *reinterpret_cast<uint4*>(tile + g * 512 + r * 16) = uint4{six[0], six[1], six[2], six[3]};
     *reinterpret_cast<uint2*>(tile + 2048 + g * 256 + r * 8) = uint2{six[4], six[5]};
   }
@@ -64,6 +64,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
 // A workgroup owns R tiles of 16 matrix rows over the whole of K; its NW waves take the tiles' runs of G steps of 128 k in turn, so that at any
 // time they read neighbouring kilobytes, D runs of a wave in flight.  The waves' sums meet in LDS and are added in the waves' order.
 // What bounds it is the stream of the matrix; the rows come from L2 again for every workgroup.
+// (8 rows of 3,584 x 18,944 in E2M3, 36.1 MB of matrix: 8.2 us, 4.4 TB/s; 37,888 x 3,584, 72 MB: 13.1 us, 5.5 TB/s; a read without work reaches 6.3.)
+
 // What the sums of 16 rows (from row m0 on) are joined to, of this thread's result: asked for in front of the stream, not behind it.
 template <int R, int NW>
 struct Joined {
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(NW * 64) void few_six_kernel(const unsigned char* _
       const int r = (i & 1) * 16 + r16;
 #pragma unroll
       for (int q = 0; q < G; ++q) {
-        const unsigned char* tile = a_codes + ((size_t)(i >> 1) * steps + min(t0 + q, steps - 1)) * 3072;
+        const unsigned char* tile = a_codes + ((size_t)(i >> 1) * steps + min(t0 + q, steps - 1)) * MX6_TILE;
         x4[q][i] = *reinterpret_cast<const uint4*>(tile + g * 512 + r * 16);
         x2[q][i] = *reinterpret_cast<const uint2*>(tile + 2048 + g * 256 + r * 8);
       }
@@ -208,7 +210,8 @@ __global__ __launch_bounds__(NW * 64) void few_six_kernel(const unsigned char* _
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     if (i) __syncthreads();
-    few_results<R, NW, PAIR>(acc[i], red, C, Joined<R, NW>(C, bias, 16 * i, M, PAIR ? 0 : N, blockIdx.x * R, epi), 16 * i, M, N, blockIdx.x * R, wid, epi, limit);
+    const Joined<R, NW> joined(C, bias, 16 * i, M, PAIR ? 0 : N, blockIdx.x * R, epi);
+    few_results<R, NW, PAIR>(acc[i], red, C, joined, 16 * i, M, N, blockIdx.x * R, wid, epi, limit);
   }
 }
 
@@ -240,7 +243,7 @@ __device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int& bm,
 template <int BM, int BN, int STAGES_>
 struct Tile {
   static constexpr int I = BM / 64, J = BN / 64;                  // blocks of 32 x 32 results of a wave (2 x 2 waves)
-  static constexpr int STAGES = STAGES_, A_ST = BM / 32 * 3072, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
+  static constexpr int STAGES = STAGES_, A_ST = BM / 32 * MX6_TILE, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
   static constexpr int PA = BM / 32 * 512, PW = BN / 16 * 256, POW = PA + PW;                  // powers of 512 k
   static constexpr int CA = BM / 32 * 3, CW = BN / 16;                                         // copies of a step: kilobytes
   static constexpr int LA = (CA + 3) / 4, LW = (CW + 3) / 4, L = LA + LW;                      // ... of a wave
@@ -295,9 +298,12 @@ __device__ __forceinline__ void leave_rows(const unsigned char* __restrict__ own
   }
 }
 
+// What bounds it: a prompt's products, the matrix cores under the card's power limit and the copies (4,096 rows, swiglu of 37,888 x 3,584, 1.11 PFLOP:
+// 350 us, 3.2 PFLOP/s; the same launch on zeros, which draw less, 265; the loop of products alone, operands in registers, 5.8 PFLOP/s on random
+// values); hundreds of rows, the latency of a workgroup's own steps (300 rows of 2,048 x 2,048: 6.3 us).
 // A workgroup of four waves (one a SIMD) takes a BM x BN tile of results, a wave a quarter of it in blocks of 32 x 32 (instruction 32x32x64).
-// A step is 128 k: its codes are copied into one of three stages as they are stored (that is the order in which the operands' lanes read them,
-// 256 bytes to 16 lanes: no two lanes of a read meet in a bank), up to three steps ahead; the powers of four steps likewise into one of two
+// A step is 128 k: its codes are copied into one of the stages as they are stored (that is the order in which the operands' lanes read them,
+// 256 bytes to 16 lanes: no two lanes of a read meet in a bank), up to STAGES steps ahead; the powers of four steps likewise into one of two
 // places.  A step runs in two halves of 64 k: while the products of one half run, the other half's operands are read; the meeting in the second
 // half says that the next step has landed and that nobody reads this one's stage any more.  Reads and copies are set between the products one
 // by one.
@@ -326,7 +332,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
 #pragma unroll
   for (int q = 0; q < TT::LA; ++q) {
     const int piece = min(q * 4 + wid, TT::CA - 1), b = piece / 3, at = piece - b * 3;
-    ga[q] = a_codes + (size_t)min(bm * (BM / 32) + b, m32 - 1) * steps * 3072 + at * 1024;
+    ga[q] = a_codes + (size_t)min(bm * (BM / 32) + b, m32 - 1) * steps * MX6_TILE + at * 1024;
     la[q] = lds0 + piece * 1024;
   }
 #pragma unroll
@@ -351,7 +357,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   }
   auto copy = [&](int q, int t, int st) {                          // q: 0 .. L - 1
     const int tc = min(t, last);
-    if (q < TT::LA) copy_kb(ga[q] + (size_t)tc * 3072, off, __builtin_amdgcn_readfirstlane(la[q] + st * TT::STAGE));
+    if (q < TT::LA) copy_kb(ga[q] + (size_t)tc * MX6_TILE, off, __builtin_amdgcn_readfirstlane(la[q] + st * TT::STAGE));
     else copy_kb(gw[q - TT::LA] + (size_t)tc * 1024, off, __builtin_amdgcn_readfirstlane(lw[q - TT::LA] + st * TT::STAGE));
   };
   auto copy_powers = [&](int q, int group) {
@@ -361,7 +367,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   };
 
   // where this lane's operands lie in a stage
-  const unsigned a16 = wm * I * 3072 + half * 512 + l32 * 16, a8 = wm * I * 3072 + 2048 + half * 256 + l32 * 8;
+  const unsigned a16 = wm * I * MX6_TILE + half * 512 + l32 * 16, a8 = wm * I * MX6_TILE + 2048 + half * 256 + l32 * 8;
   const unsigned hi = l32 >> 4, r16 = lane & 15;
   const unsigned wb = TT::A_ST + wn * J * 2048 + hi * 1024 + half * 256 + r16 * 16;
   const unsigned pa = TT::STAGES * TT::STAGE + wm * I * 512 + half * 128 + l32 * 4;
@@ -380,8 +386,8 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   auto read = [&](int i, auto H, int st, bool begins, int group) {
     constexpr int h = decltype(H)::value;
     if (i < I) {
-      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + i * 3072 + h * 1024);
-      const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + i * 3072 + h * 512);
+      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + i * MX6_TILE + h * 1024);
+      const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + i * MX6_TILE + h * 512);
       fa[h][i] = intx8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, 0, 0};
       if (begins) sa[h][i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + i * 512 + h * 256);
     } else {
@@ -457,7 +463,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   __syncthreads();                                                 // (nobody reads the stages any more)
   // D[n][m]: m = lane % 32, n = 8 (r / 4) + 4 (lane / 32) + r % 4 (gate rows the first 16, up rows the others): a lane holds four neighbouring
   // results of a row.  32 rows at a time by way of LDS, so that a store takes 16 bytes a lane and whole lines of a row (straight from the
-  // registers, four bytes a lane: 63 us for 2,048 rows of 4,608 x 3,584 that take 35 so).
+  // registers, four bytes a lane: 63 us for 2,048 rows of 4,608 x 3,584 that take 34 so).
   unsigned char* own = smem + wid * 32 * TT::ROW;
   const bool once = leaves_once((size_t)M * N * (PAIR || epi == EPI_BF16 ? 2 : 4));
 #pragma unroll
@@ -552,7 +558,7 @@ enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 4 };
 struct Plan { int form, splits, groups; };
 
 // What a tile kernel and the sum behind it take, in microseconds: fixed, by the workgroups of the fullest CU, by their steps (one workgroup's
-// latency, or all of them by their products), by what is written.  Least squares over 1,066 products of 65 to 16,384 rows, 896 to 152,064 matrix rows
+// latency, or all of them by their products), by what is written.  Least squares over 971 timings of 88 products of 65 to 16,384 rows, 896 to 152,064 matrix rows
 // and K of 896 to 18,944 (7.6 % rms off); the plan that it finds least takes 0.5 % longer than the best on the average, 12 % at most.
 struct TileForm { int m, n; double step, step_each, fixed, each; };
 constexpr TileForm TILE_FORMS[N_TILE_FORMS] = {{256, 256, 0.617, 0.617, 8.2, 7.0}, {256, 128, 0.550, 0.372, 7.6, 1.8},
@@ -576,8 +582,8 @@ static Plan make_plan(int M, int w16, int steps, bool whole, bool pair, double o
     const long blocks = w16 > n_cu ? (w16 + 1) / 2 : w16, u = (blocks + n_cu - 1) / n_cu * steps;
     return Plan{whole && (M <= 4 || u <= (M <= 8 ? 80 : 24)) ? FEW_RAW : FEW_SIX, 1, groups};
   }
-  // 17 to 64 rows: `few_six_kernel` by the steps of a CU's tiles (two and four tiles of rows: 6.5 + 0.054 us a step, 7.2 + 0.098; 90 products within
-  // 15 %) against the tiles: 32 rows, 3,584 x 18,944 14.7 / 17.4 us; 64 rows 22.0 / 18.2, swiglu of 37,888 x 3,584 36.9 / 20.8.
+  // 17 to 64 rows: `few_six_kernel` by the steps of a CU's tiles (two and four tiles of rows: 6.5 + 0.054 us a step, 7.2 + 0.098; 69 products, 7 % rms off,
+  // 17 % at most) against the tiles: 32 rows, 3,584 x 18,944 14.7 / 17.4 us; 64 rows 22.0 / 18.2, swiglu of 37,888 x 3,584 36.9 / 20.8.
   const int run = w16 > n_cu || pair ? 2 : 1;
   const double few = (double)(((w16 + run - 1) / run + n_cu - 1) / n_cu) * run * steps;
   Plan best{FEW_SIX, 1, groups};
@@ -605,7 +611,7 @@ MF_API int mf_mx4_plan(int M, int N, int K, int epi, int whole, int n_cu, long l
   const Plan p = make_plan(M, (int)w16, (int)steps, whole, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
   out[0] = p.form;
   out[1] = p.splits;
-  out[2] = p.form == FEW_RAW ? 0 : m32 * (steps * 3072 + groups * 512);
+  out[2] = p.form == FEW_RAW ? 0 : m32 * (steps * MX6_TILE + groups * 512);
   out[3] = p.splits > 1 ? (long long)p.splits * M * w16 * 16 : 0;
   return 0;
 }
@@ -618,7 +624,7 @@ static int launch_tiles(const unsigned char* six, const void* codes, const void*
   if (e != hipSuccess) return (int)e;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (w16 * 16 + BN - 1) / BN;
   tile_kernel<BM, BN, STAGES, PER_CU, PAIR><<<dim3(tiles_m * tiles_n, p.splits), 256, TT::LDS, stream>>>(
-      six, six + (size_t)m32 * steps * 3072, (const unsigned char*)codes, (const unsigned char*)powers, bias, C, p.splits > 1 ? part : nullptr, M, N,
+      six, six + (size_t)m32 * steps * MX6_TILE, (const unsigned char*)codes, (const unsigned char*)powers, bias, C, p.splits > 1 ? part : nullptr, M, N,
       m32, w16, steps, groups, tiles_m, tiles_n, p.groups, epi, limit);
   return mf_launch_status();
 }
@@ -633,7 +639,8 @@ static int with_tiles(int epi, int w16, int n_cu, F run) {
 }
 
 // C [M][N] (float32, added to where epi is EPI_ACC_F32, or bfloat16) from x [M][K] (bfloat16 or float32) and the stored [N][K]; EPI_SWIGLU: C is
-// [M][N] bfloat16 and the matrix holds N gate rows and N up rows, tile by tile in turn (limit above 0: the clamped gate with it).  scratch: as `mf_mx4_plan` says, 16-byte aligned.
+// [M][N] bfloat16 and the matrix holds N gate rows and N up rows, tile by tile in turn (limit above 0: the clamped gate with it).  scratch: as
+// `mf_mx4_plan` says, 16-byte aligned.
 MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const void* powers, const float* bias, void* C, void* scratch, float* part,
                          int M, int N, int K, int epi, float limit, int n_cu, hipStream_t stream) {
   long long sizes[4];
@@ -642,7 +649,7 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
   if (bad) return bad;
   const int w16 = (epi == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
   const Plan p = make_plan(M, w16, steps, vec, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
-  unsigned* a_powers = (unsigned*)((unsigned char*)scratch + (size_t)m32 * steps * 3072);
+  unsigned* a_powers = (unsigned*)((unsigned char*)scratch + (size_t)m32 * steps * MX6_TILE);
   if (p.form == FEW_RAW)
     return with_tiles(epi, w16, n_cu, [&](auto R0, auto PAIR) {
       constexpr int R = decltype(R0)::value;

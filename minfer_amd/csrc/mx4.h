@@ -31,6 +31,7 @@ typedef float floatx2 __attribute__((ext_vector_type(2)));
 
 constexpr unsigned MX_E2M1_CARRY = 0x1FFFFF, MX_E2M3_CARRY = 0x0FFFFF;       // mantissas above 1.75, above 1.875
 constexpr int MX_FP6 = 2, MX_FP4 = 4;                                        // operand formats of the matrix instructions
+constexpr int MX6_TILE = 3 * 1024;                                           // bytes of 32 rows' 128 values in E2M3
 
 // the stored power of a block whose largest magnitude has these bits (of a 32-bit float, without the sign)
 __device__ __forceinline__ unsigned mx_power(unsigned largest, unsigned carry) {
@@ -92,7 +93,7 @@ __device__ __forceinline__ void mx_load_words(const uint4* from, unsigned (&word
 
 // Four rows' 512 values from k0 on, by way of LDS: asked for in the order of memory, 16 bytes a lane (WHOLE: the rows begin at multiples of 16
 // bytes) or a value a lane; zeros past row m and past k.  A block of 32 values lies there as pieces of 16 bytes in a rotated order, so that
-// eight lanes that read the same piece of eight neighbouring blocks meet in no bank.  One wave's; `mx_staged` is for the same wave.
+// eight lanes that read the same piece of eight neighbouring blocks meet in no bank.  One wave's: nobody else reads it.
 template <typename T>
 struct MxStage {
   static constexpr int PIECES = 2 * sizeof(T), PER = 16 / sizeof(T);            // of a block; values of a piece

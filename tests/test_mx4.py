@@ -47,7 +47,7 @@ def test_every_plan_covers_its_product(m, n, k):
         assert 1 <= splits <= groups and (splits - 1) * per < groups <= splits * per
         assert parts == (splits * m * w16 * 16 if splits > 1 else 0)
         assert m <= 16 and whole or form > 0
-        assert six == (0 if form == 0 else -(-m // 32) * (steps * 3072 + groups * 512))
+        assert six == (0 if form == 0 else -(-m // 32) * (steps * 3 * 1024 + groups * 512))
 
 
 def test_weights_option():
