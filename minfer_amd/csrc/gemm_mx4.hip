@@ -242,7 +242,7 @@ __device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int& bm,
 
 template <int BM, int BN, int STAGES_>
 struct Tile {
-  static constexpr int I = BM / 64, J = BN / 64;                  // blocks of 32 x 32 results of a wave (2 x 2 waves)
+  static constexpr int I = BM / 32, J = BN / 32;                  // blocks of 16 x 16 results of a wave (2 x 2 waves)
   static constexpr int STAGES = STAGES_, A_ST = BM / 32 * MX6_TILE, W_ST = BN / 16 * 1024, STAGE = A_ST + W_ST;
   static constexpr int PA = BM / 32 * 512, PW = BN / 16 * 256, POW = PA + PW;                  // powers of 512 k
   static constexpr int CA = BM / 32 * 3, CW = BN / 16;                                         // copies of a step: kilobytes
@@ -298,15 +298,18 @@ __device__ __forceinline__ void leave_rows(const unsigned char* __restrict__ own
   }
 }
 
-// What bounds it: a prompt's products, the matrix cores under the card's power limit and the copies (4,096 rows, swiglu of 37,888 x 3,584, 1.11 PFLOP:
-// 350 us, 3.2 PFLOP/s; the same launch on zeros, which draw less, 265; the loop of products alone, operands in registers, 5.8 PFLOP/s on random
-// values); hundreds of rows, the latency of a workgroup's own steps (300 rows of 2,048 x 2,048: 6.3 us).
-// A workgroup of four waves (one a SIMD) takes a BM x BN tile of results, a wave a quarter of it in blocks of 32 x 32 (instruction 32x32x64).
+// A workgroup of four waves (one a SIMD) takes a BM x BN tile of results, a wave a quarter of it in blocks of 16 x 16.
 // A step is 128 k: its codes are copied into one of the stages as they are stored (that is the order in which the operands' lanes read them,
 // 256 bytes to 16 lanes: no two lanes of a read meet in a bank), up to STAGES steps ahead; the powers of four steps likewise into one of two
-// places.  A step runs in two halves of 64 k: while the products of one half run, the other half's operands are read; the meeting in the second
-// half says that the next step has landed and that nobody reads this one's stage any more.  Reads and copies are set between the products one
-// by one.
+// places.  A step's products run in two halves, the upper half of the wave's rows and the lower: beside the first run the reads of the second's
+// rows, beside the second those of the next step's matrix and first rows, so that of the rows one step's operands are held and of the matrix
+// two.  The meeting in the second half says that the next step has landed and that nobody reads this one's stage any more.  Reads and copies are
+// set between the products one by one.
+// What bounds it: a prompt's products, the card's power and what is not beside products, a tile's first copies and its stores (4,096 rows, swiglu of
+// 37,888 x 3,584, 1.11 PFLOP: 346 us, 3.2 PFLOP/s; the same launch on zeros, which draw less, an eighth less; the products alone from registers
+// 6.9 PFLOP/s on values as they are here, 9.7 on zeros); hundreds of rows, the latency of a workgroup's own steps (300 rows of 2,048 x 2,048: 6.3 us).
+// Why 16x16x128 and not 32x32x64: under the power limit the products alone run at 6.9 PFLOP/s instead of 5.9 (the whole launch above in 353 us
+// instead of 363, with the reads the same).
 template <int BM, int BN, int STAGES, int PER_CU, bool PAIR>
 __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* __restrict__ a_codes, const unsigned char* __restrict__ a_powers,
                                                       const unsigned char* __restrict__ w_codes, const unsigned char* __restrict__ w_powers,
@@ -320,7 +323,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   tile_of_block(tiles_m, tiles_n, bm, bn);
   const int g0 = blockIdx.y * groups_per_part, g1 = min(g0 + groups_per_part, groups);
   const int t0 = g0 * 4, t1 = min(g1 * 4, steps), last = t1 - 1;
-  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid >> 1, wn = wid & 1;
   const unsigned lds0 = (unsigned)(uintptr_t)smem;
@@ -345,9 +348,9 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   for (int q = 0; q < TT::LP; ++q) {
     const int piece = min(q * 4 + wid, TT::NPA + TT::NPW - 1);
     if (piece < TT::NPA) {
-      const int b0 = min(bm * (BM / 32) + piece * 2, m32 - 1), b = min(bm * (BM / 32) + piece * 2 + half, m32 - 1);
+      const int b0 = min(bm * (BM / 32) + piece * 2, m32 - 1), b = min(bm * (BM / 32) + piece * 2 + (lane >> 5), m32 - 1);
       gp[q] = a_powers + (size_t)b0 * groups * 512;
-      off_p[q] = (unsigned)(b - b0) * groups * 512 + l32 * 16;
+      off_p[q] = (unsigned)(b - b0) * groups * 512 + (lane & 31) * 16;
     } else {
       const int pw = piece - TT::NPA, b0 = min(bn * (BN / 16) + pw * 4, w16 - 1), b = min(bn * (BN / 16) + pw * 4 + (lane >> 4), w16 - 1);
       gp[q] = w_powers + (size_t)b0 * groups * 256;
@@ -367,41 +370,41 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   };
 
   // where this lane's operands lie in a stage
-  const unsigned a16 = wm * I * MX6_TILE + half * 512 + l32 * 16, a8 = wm * I * MX6_TILE + 2048 + half * 256 + l32 * 8;
-  const unsigned hi = l32 >> 4, r16 = lane & 15;
-  const unsigned wb = TT::A_ST + wn * J * 2048 + hi * 1024 + half * 256 + r16 * 16;
-  const unsigned pa = TT::STAGES * TT::STAGE + wm * I * 512 + half * 128 + l32 * 4;
-  const unsigned pw = TT::STAGES * TT::STAGE + TT::PA + wn * J * 512 + hi * 256 + half * 64 + r16 * 4;
+  const int r16 = lane & 15, g = lane >> 4;
+  const unsigned a16 = wm * (I / 2) * MX6_TILE + g * 512 + r16 * 16, a8 = wm * (I / 2) * MX6_TILE + 2048 + g * 256 + r16 * 8;
+  const unsigned wb = TT::A_ST + wn * J * 1024 + lane * 16;
+  const unsigned pa = TT::STAGES * TT::STAGE + wm * (I / 2) * 512 + g * 128 + r16 * 4;
+  const unsigned pw = TT::STAGES * TT::STAGE + TT::PA + wn * J * 256 + lane * 4;
 
-  floatx16 acc[I][J];
+  floatx4 acc[I][J];
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  intx8 fa[2][I], fw[2][J];
-  int sa[2][I], sw[2][J];
-  // read i of a half's operands: rows i, then matrix rows i - I, and their powers where a group of four steps begins
-  auto read = [&](int i, auto H, int st, bool begins, int group) {
-    constexpr int h = decltype(H)::value;
-    if (i < I) {
-      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + i * MX6_TILE + h * 1024);
-      const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + i * MX6_TILE + h * 512);
-      fa[h][i] = intx8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, 0, 0};
-      if (begins) sa[h][i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + i * 512 + h * 256);
-    } else {
-      const int j = i - I;
-      const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + wb + j * 2048 + h * 512);
-      fw[h][j] = mx4_operand(x);
-      if (begins) sw[h][j] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pw + j * 512 + h * 128);
-    }
+    for (int j = 0; j < J; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  intx8 fa[I], fw[2][J];
+  int sa[I], sw[J], sw_next[J];
+  // the operands of rows block i, of matrix block j (those of two steps in a row stand side by side), and their powers where a group begins
+  auto read_rows = [&](int i, int st, bool begins, int group) {
+    const int tile = i / 2, half = i % 2;
+    const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + tile * MX6_TILE + half * 256);
+    const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + tile * MX6_TILE + half * 128);
+    fa[i] = intx8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, 0, 0};
+    if (begins) sa[i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + tile * 512 + half * 64);
   };
-  using H0 = std::integral_constant<int, 0>;
-  using H1 = std::integral_constant<int, 1>;
+  auto read_matrix = [&](int j, int side, int st, bool begins, int group) {
+    fw[side][j] = mx4_operand(*reinterpret_cast<const uint4*>(smem + st * TT::STAGE + wb + j * 1024));
+    if (begins) sw_next[j] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pw + j * 256);
+  };
+  // read z of what a step's first half needs: rows 0, the matrix, the other rows of the half
+  auto read_first = [&](int z, int side, int st, bool begins, int group) {
+    if (z == 0) read_rows(0, st, begins, group);
+    else if (z <= J) read_matrix(z - 1, side, st, begins, group);
+    else read_rows(z - J, st, begins, group);
+  };
   // products of a half, in front of its meeting and behind it; operand reads of a half; copies of a step that are set out behind the meeting of
   // the step three before it (the rest: in the first half of the next one)
-  constexpr int NM = I * J, BEFORE = NM / 4, BEHIND = NM - BEFORE, READS = I + J, EARLY = STAGES == 2 ? TT::L : (TT::L * BEHIND + NM + BEHIND - 1) / (NM + BEHIND);
+  constexpr int NM = I / 2 * J, BEFORE = NM / 4, BEHIND = NM - BEFORE, FIRST = I / 2 + J;
+  constexpr int EARLY = STAGES == 2 ? TT::L : (TT::L * BEHIND + NM + BEHIND - 1) / (NM + BEHIND);
 
 #pragma unroll
   for (int q = 0; q < TT::LP; ++q) copy_powers(q, g0);
@@ -411,7 +414,9 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
     for (int q = 0; q < (t == STAGES - 1 ? EARLY : TT::L); ++q) copy(q, t0 + t, t);
   wait_and_meet<(STAGES - 2) * TT::L + EARLY>();
 #pragma unroll
-  for (int i = 0; i < I + J; ++i) read(i, H0{}, 0, true, g0);
+  for (int z = 0; z < FIRST; ++z) read_first(z, 0, 0, true, g0);
+#pragma unroll
+  for (int j = 0; j < J; ++j) sw[j] = sw_next[j];
 
   int st = 0;
   auto step = [&](int t, int group, auto S) {
@@ -421,9 +426,9 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
       const int i = q / J, j = q % J;
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[0][j], fa[0][i], acc[i][j], MX_FP4, MX_FP6, s, sw[0][j], s, sa[0][i]);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[s & 1][j], fa[i], acc[i][j], MX_FP4, MX_FP6, s, sw[j], s, sa[i]);
 #pragma unroll
-      for (int z = q * READS / NM; z < (q + 1) * READS / NM; ++z) read(z, H1{}, st, s == 0, group);
+      for (int z = q * (I / 2) / NM; z < (q + 1) * (I / 2) / NM; ++z) read_rows(I / 2 + z, st, s == 0, group);
 #pragma unroll
       for (int z = q * (TT::L - EARLY) / NM; z < (q + 1) * (TT::L - EARLY) / NM; ++z) copy(EARLY + z, t + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
       __builtin_amdgcn_sched_barrier(0);
@@ -433,13 +438,13 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
     constexpr int FLIGHT = (STAGES - 2) * TT::L + (s == 1 ? TT::LP : 0), COPIES = EARLY + (s == 0 ? TT::LP : 0);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
-      const int i = q / J, j = q % J;
+      const int i = I / 2 + q / J, j = q % J;
       if (q == BEFORE) wait_and_meet<FLIGHT>();
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[1][j], fa[1][i], acc[i][j], MX_FP4, MX_FP6, s, sw[1][j], s, sa[1][i]);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[s & 1][j], fa[i], acc[i][j], MX_FP4, MX_FP6, s, sw[j], s, sa[i]);
       if (q >= BEFORE) {
         const int b = q - BEFORE;
 #pragma unroll
-        for (int z = b * READS / BEHIND; z < (b + 1) * READS / BEHIND; ++z) read(z, H0{}, next, s == 3, group + 1);
+        for (int z = b * FIRST / BEHIND; z < (b + 1) * FIRST / BEHIND; ++z) read_first(z, (s + 1) & 1, next, s == 3, group + 1);
 #pragma unroll
         for (int z = b * COPIES / BEHIND; z < (b + 1) * COPIES / BEHIND; ++z) {
           if (z < EARLY) copy(z, t + STAGES, st);
@@ -449,6 +454,10 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
       __builtin_amdgcn_sched_barrier(0);
     }
     st = next;
+    if constexpr (s == 3) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) sw[j] = sw_next[j];
+    }
   };
   for (int group = g0; group < g1; ++group) {
     const int t = group * 4;
@@ -461,58 +470,61 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   __syncthreads();                                                 // (nobody reads the stages any more)
-  // D[n][m]: m = lane % 32, n = 8 (r / 4) + 4 (lane / 32) + r % 4 (gate rows the first 16, up rows the others): a lane holds four neighbouring
-  // results of a row.  32 rows at a time by way of LDS, so that a store takes 16 bytes a lane and whole lines of a row (straight from the
-  // registers, four bytes a lane: 63 us for 2,048 rows of 4,608 x 3,584 that take 34 so).
+  // D[n][m]: m = lane % 16, n = 4 (lane / 16) + r (a gate's block, then its up's): a lane holds four neighbouring results of a row.  32 rows at a
+  // time by way of LDS, so that a store takes 16 bytes a lane and whole lines of a row (straight from the registers, four bytes a lane: 63 us
+  // for 2,048 rows of 4,608 x 3,584 that take 34 so).
   unsigned char* own = smem + wid * 32 * TT::ROW;
   const bool once = leaves_once((size_t)M * N * (PAIR || epi == EPI_BF16 ? 2 : 4));
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const int m_first = bm * BM + wm * I * 32 + i * 32;
+  for (int i = 0; i < I / 2; ++i) {
+    const int m_first = bm * BM + (wm * (I / 2) + i) * 32;
     if (m_first >= M) continue;
     const int rows = min(32, M - m_first);
     auto floats = [&]() {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<floatx4*>(own + l32 * TT::ROW + (j * 32 + q * 8 + half * 4) * 4) =
-              floatx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        for (int j = 0; j < J; ++j) *reinterpret_cast<floatx4*>(own + (h * 16 + r16) * TT::ROW + (j * 16 + g * 4) * 4) = acc[2 * i + h][j];
     };
     if (part) {
       floats();
       __builtin_amdgcn_wave_barrier();
-      leave_rows<J * 32, EPI_F32>(own, TT::ROW, part + (size_t)blockIdx.y * M * (w16 * 16), m_first, rows, bn * BN + wn * J * 32, w16 * 16, nullptr, false, lane);
+      leave_rows<J * 16, EPI_F32>(own, TT::ROW, part + (size_t)blockIdx.y * M * (w16 * 16), m_first, rows, bn * BN + wn * J * 16, w16 * 16, nullptr, false, lane);
     } else if constexpr (PAIR) {
+      auto gates = [&](auto gate) {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          bf16x4 y;
+          for (int j = 0; j < J; j += 2) {
+            bf16x4 y;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) y[x] = (bf16)gate_mul(acc[i][j][4 * q + x], acc[i][j][8 + 4 * q + x], limit);
-          *reinterpret_cast<bf16x4*>(own + l32 * TT::ROW + (j * 16 + q * 8 + half * 4) * 2) = y;
-        }
+            for (int x = 0; x < 4; ++x) y[x] = (bf16)gate(acc[2 * i + h][j][x], acc[2 * i + h][j + 1][x]);
+            *reinterpret_cast<bf16x4*>(own + (h * 16 + r16) * TT::ROW + (j * 8 + g * 4) * 2) = y;
+          }
+      };
+      // (the limit is asked about once, not for every result: 4,096 rows of 37,888 x 3,584 335 us, 327 so)
+      if (limit > 0.f) gates([=](float gate, float up) { return clamped_gate(gate, up, limit); });
+      else gates([](float gate, float up) { return silu_mul(gate, up); });
       __builtin_amdgcn_wave_barrier();
-      leave_rows<J * 16, EPI_BF16>(own, TT::ROW, C, m_first, rows, bn * (BN / 2) + wn * J * 16, N, nullptr, once, lane);
+      leave_rows<J * 8, EPI_BF16>(own, TT::ROW, C, m_first, rows, bn * (BN / 2) + wn * J * 8, N, nullptr, once, lane);
     } else if (epi == EPI_BF16) {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = bn * BN + wn * J * 32 + j * 32 + q * 8 + half * 4;
+        for (int j = 0; j < J; ++j) {
+          const int n = bn * BN + (wn * J + j) * 16 + g * 4;
           bf16x4 y;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) y[x] = (bf16)(acc[i][j][4 * q + x] + (bias && n + x < N ? bias[n + x] : 0.f));
-          *reinterpret_cast<bf16x4*>(own + l32 * TT::ROW + (j * 32 + q * 8 + half * 4) * 2) = y;
+          for (int x = 0; x < 4; ++x) y[x] = (bf16)(acc[2 * i + h][j][x] + (bias && n + x < N ? bias[n + x] : 0.f));
+          *reinterpret_cast<bf16x4*>(own + (h * 16 + r16) * TT::ROW + (j * 16 + g * 4) * 2) = y;
         }
       __builtin_amdgcn_wave_barrier();
-      leave_rows<J * 32, EPI_BF16>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 32, N, nullptr, once, lane);
+      leave_rows<J * 16, EPI_BF16>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 16, N, nullptr, once, lane);
     } else {
       floats();
       __builtin_amdgcn_wave_barrier();
-      if (epi == EPI_ACC_F32) leave_rows<J * 32, EPI_ACC_F32>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 32, N, bias, false, lane);
-      else leave_rows<J * 32, EPI_F32>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 32, N, bias, once, lane);
+      if (epi == EPI_ACC_F32) leave_rows<J * 16, EPI_ACC_F32>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 16, N, bias, false, lane);
+      else leave_rows<J * 16, EPI_F32>(own, TT::ROW, C, m_first, rows, bn * BN + wn * J * 16, N, bias, once, lane);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -557,17 +569,18 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
 enum { FEW_RAW = 0, FEW_SIX = 1, TILES = 2, N_TILE_FORMS = 4 };
 struct Plan { int form, splits, groups; };
 
-// What a tile kernel and the sum behind it take, in microseconds: fixed, by the workgroups of the fullest CU, by their steps (one workgroup's
-// latency, or all of them by their products), by what is written.  Least squares over 971 timings of 88 products of 65 to 16,384 rows, 896 to 152,064 matrix rows
-// and K of 896 to 18,944 (7.6 % rms off); the plan that it finds least takes 0.5 % longer than the best on the average, 12 % at most.
-struct TileForm { int m, n; double step, step_each, fixed, each; };
-constexpr TileForm TILE_FORMS[N_TILE_FORMS] = {{256, 256, 0.617, 0.617, 8.2, 7.0}, {256, 128, 0.550, 0.372, 7.6, 1.8},
-                                               {128, 128, 0.245, 0.219, 7.2, 1.04}, {64, 64, 0.166, 0.108, 6.1, 0.62}};
-static double tile_cost(int f, int M, int w16, int steps, int splits, double out_bytes, int n_cu) {
+// What a tile kernel and the sum behind it take, in microseconds: fixed, by the workgroups of the fullest CU (with gates a little more), by their
+// steps (one workgroup's latency, or all of them by their products), by what is written.  Fitted to 971 timings of 88 products of 65 to 16,384
+// rows, 896 to 152,064 matrix rows and K of 896 to 18,944 (7.6 % rms off), then moved until the plans it finds least came close to the best:
+// 0.2 % longer on the average, 4 % at most.
+struct TileForm { int m, n; double step, step_each, fixed, each, gates; };
+constexpr TileForm TILE_FORMS[N_TILE_FORMS] = {{256, 256, 0.743, 0.717, 9.0, 4.75, 1.36}, {256, 128, 0.594, 0.383, 6.55, 1.96, 0.50},
+                                               {128, 128, 0.290, 0.217, 6.8, 1.11, 0.28}, {64, 64, 0.154, 0.103, 6.2, 0.64, 0.0}};
+static double tile_cost(int f, int M, int w16, int steps, int splits, bool pair, double out_bytes, int n_cu) {
   const TileForm& t = TILE_FORMS[f];
   const long tiles = (long)((M + t.m - 1) / t.m) * ((w16 * 16L + t.n - 1) / t.n) * splits, each = (tiles + n_cu - 1) / n_cu;
-  const double written = splits > 1 ? 2.9 + 0.97e-6 * M * w16 * 16 * splits + 0.27e-6 * out_bytes : 0.195e-6 * out_bytes;
-  return t.fixed + t.each * each + steps * std::max(t.step, t.step_each * each) + written;
+  const double written = splits > 1 ? 3.1 + 1.22e-6 * M * w16 * 16 * splits + 0.139e-6 * out_bytes : 0.209e-6 * out_bytes;
+  return t.fixed + (t.each + (pair && splits == 1 ? t.gates : 0.)) * each + steps * std::max(t.step, t.step_each * each) + written;
 }
 
 // `whole`: rows of x whose 16-byte pieces begin at multiples of 16 bytes (as they come, `few_kernel` reads no others).
@@ -592,7 +605,7 @@ static Plan make_plan(int M, int w16, int steps, bool whole, bool pair, double o
     for (int s = 1; s <= std::min(groups, 16); ++s) {
       const int per = (groups + s - 1) / s;
       if ((groups + per - 1) / per != s) continue;
-      const double cost = tile_cost(f, M, w16, std::min(per * 4, steps), s, out_bytes, n_cu);
+      const double cost = tile_cost(f, M, w16, std::min(per * 4, steps), s, pair, out_bytes, n_cu);
       if (cost < least) {
         least = cost;
         best = Plan{TILES + f, s, per};
