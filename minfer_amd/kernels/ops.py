@@ -2275,7 +2275,7 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias:
     """out (+)= x' W'^T (+ bias): W' the matrix `[n][k]` that `codes`, `powers` hold in microscaled 4-bit numbers (`mx4_quantise`), x' the rows
     of `x` `[m][k]` (float32 or bfloat16) in microscaled 6-bit ones (E2M3: blocks of 32, the smallest power of two with which the largest magnitude is
     at most 7.5, the nearest value, ties to even), which the product makes on its way.  Sums and `bias` are 32-bit; `out` `[m][n]` is float32, or
-    bfloat16 where it is stored.  A row of x with an infinity or a NaN gives NaN."""
+    bfloat16 where it is stored, and shares no memory with x.  A row of x with an infinity or a NaN gives NaN."""
     _need(x, "mx4_linear.x", _FLOATS)
     _need(out, "mx4_linear.out", _FLOATS)
     if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0]:
@@ -2304,7 +2304,7 @@ def mx4_linear_swiglu(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor
     x' as in `mx4_linear`, `out` bfloat16 `[m][f]`.  A `limit` above 0: the clamped form of `swiglu` with it."""
     _need(x, "mx4_linear_swiglu.x", _FLOATS)
     _need(out, "mx4_linear_swiglu.out", torch.bfloat16)
-    if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0] or limit < 0:
+    if x.dim() != 2 or out.dim() != 2 or out.shape[0] != x.shape[0] or not limit >= 0:
         raise KernelError(f"mx4_linear_swiglu: x {tuple(x.shape)}, out {tuple(out.shape)}, limit {limit}")
     m, k = x.shape
     f = out.shape[1]

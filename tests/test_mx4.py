@@ -50,6 +50,14 @@ def test_every_plan_covers_its_product(m, n, k):
         assert six == (0 if form == 0 else -(-m // 32) * (steps * 3 * 1024 + groups * 512))
 
 
+@pytest.mark.parametrize("limit", [-1.0, float("nan")])
+def test_a_limit_that_is_none(limit, monkeypatch):
+    monkeypatch.setattr(ops, "_need", lambda *a: None)
+    codes, powers = (torch.zeros(s, dtype=torch.uint8) for s in ops._mx4_pair_shapes(32, 64))
+    with pytest.raises(ops.KernelError, match="limit"):
+        ops.mx4_linear_swiglu(torch.zeros((3, 64)), codes, powers, torch.zeros((3, 32), dtype=torch.bfloat16), limit=limit)
+
+
 def test_weights_option():
     from minfer_amd import config_from_dict
     from minfer_amd.engine.model import DecoderModel

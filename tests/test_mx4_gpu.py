@@ -127,6 +127,50 @@ def test_linear_swiglu(m, f, k):
     within(out, want, bound + half_step(BF16) * (want.abs() + bound) + 1e-37)
 
 
+# (kernel, whether K is cut over blocks, m, n, k): each tile kernel at sizes where the plan takes it, with tiles that end outside
+TILED = [(2, False, 6404, 4408, 5899), (3, False, 396, 8626, 64), (3, True, 1625, 2795, 15905), (4, False, 2778, 720, 84), (4, True, 720, 1508, 8730),
+         (5, False, 46, 65, 67), (5, True, 66, 72, 3114)]
+TILED_GATES = [(2, False, 3484, 4102, 6683), (3, False, 772, 2662, 66), (3, True, 1297, 1535, 17507), (4, False, 196, 6430, 64),
+               (4, True, 257, 804, 12727), (5, False, 70, 333, 200), (5, True, 42, 70, 3383)]
+
+
+def planned(kernel, cut, m, n, k, epi):
+    from minfer_amd.kernels import ops
+    if ops.cu_count() == 256:
+        form, parts, _, _ = ops._mx4_plan(m, n, k, epi, True, 256)
+        assert (form, parts > 1) == (kernel, cut)
+
+
+@pytest.mark.parametrize("kernel,cut,m,n,k", TILED)
+def test_linear_in_every_tile_kernel(kernel, cut, m, n, k):
+    from minfer_amd.kernels import ops
+    planned(kernel, cut, m, n, k, ops.EPI_ACC_F32)
+    x, bias, before = normal((m, k), m + n), normal((n,), 7, F32), normal((m, n), 8, F32)
+    codes, powers = quantised(normal((n, k), n + k, std=0.05))
+    want, size = plain.product(x, plain.read(codes, powers, n, k))
+    for add, out_dtype in ((True, F32), (False, BF16)):
+        out = before.clone() if add else torch.full((m, n), float("nan"), dtype=out_dtype, device=DEV)
+        ops.mx4_linear(x, codes, powers, bias, out, accumulate=add)
+        bound = plain.sum_error(k, size + bias.double().abs() + (before.double().abs() if add else 0))
+        whole = want + bias.double() + (before.double() if add else 0)
+        within(out, whole, bound + half_step(out_dtype) * (whole.abs() + bound) + 1e-37)
+
+
+@pytest.mark.parametrize("kernel,cut,m,f,k", TILED_GATES)
+def test_linear_swiglu_in_every_tile_kernel(kernel, cut, m, f, k):
+    from minfer_amd.kernels import ops
+    planned(kernel, cut, m, f, k, ops.EPI_SWIGLU)
+    x = normal((m, k), m + f)
+    gate, up = quantised(normal((f, k), 1, std=0.05)), quantised(normal((f, k), 2, std=0.05))
+    out = torch.full((m, f), float("nan"), dtype=BF16, device=DEV)
+    ops.mx4_linear_swiglu(x, ops.mx4_pairs(gate[0], up[0]), ops.mx4_pairs(gate[1], up[1]), out)
+    (g, g_size), (u, u_size) = (plain.product(x, plain.read(*t, f, k)) for t in (gate, up))
+    dg, du = plain.sum_error(k, g_size), plain.sum_error(k, u_size)
+    want = plain.silu(g) * u
+    bound = 1.1 * dg * (u.abs() + du) + g.abs() * du + (g.abs() + 16) * 2.0 ** -22 * want.abs()        # (as in test_linear_swiglu)
+    within(out, want, bound + half_step(BF16) * (want.abs() + bound) + 1e-37)
+
+
 @pytest.mark.parametrize("m", [7, 48, 130])
 def test_linear_swiglu_clamped(m):
     from minfer_amd.kernels import ops
@@ -330,6 +374,24 @@ def test_experts_that_hand_on(dtype):
     out = torch.zeros((3, k), device=DEV)
     ops.mx4_moe_sparse(x, *layer, chosen, weights, out, f, act=1, hands_on=True)
     within(out, want, bound + 4 * half_step(F32) * (want.abs() + x.double().abs()) + 1e-37)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens", [2, 6, 16])
+def test_experts_of_rows_that_begin_anywhere(tokens, dtype):
+    """x, outputs and the rows handed on at odd addresses: the same bits as from aligned ones."""
+    from minfer_amd.kernels import ops
+    e, f, k = 4, 96, 168
+    layer, _ = experts(e, f, k, 5)
+    gen = torch.Generator().manual_seed(tokens)
+    chosen = torch.randint(0, e + 2, (tokens, 3), generator=gen).to(torch.int32).to(DEV)
+    weights = torch.rand((tokens, 3), generator=gen).to(DEV)
+    x = normal((tokens, k), 6, dtype)
+    outs = []
+    for rows, out in ((x, torch.zeros((tokens, k), device=DEV)), (misaligned(x), misaligned(torch.zeros((tokens, k), device=DEV)))):
+        ops.mx4_moe_sparse(rows, *layer, chosen, weights, out, f, act=1, hands_on=True)
+        outs.append(out)
+    assert outs[0].any(1).all() and torch.equal(*outs)
 
 
 # ------------------------------------------------------------------ as they are used
