@@ -700,17 +700,16 @@ MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const vo
       if (M <= 32) return run(std::integral_constant<int, 2>{});
       return run(std::integral_constant<int, 4>{});
     });
-  auto tiles = [&](auto BM, auto BN, auto STAGES, auto PER_CU, auto PAIR) {
-    return launch_tiles<decltype(BM)::value, decltype(BN)::value, decltype(STAGES)::value, decltype(PER_CU)::value, decltype(PAIR)::value>((const unsigned char*)scratch, codes, powers, bias, C, part, M, N,
-                                                                                     m32, w16, steps, groups, p, epi, limit, stream);
-  };
-  auto choose = [&](auto PAIR) {
-    using std::integral_constant;
+  auto choose = [&](auto PAIR0) {
+    constexpr bool PAIR = decltype(PAIR0)::value;
+    auto tiles = [&](auto launch) {
+      return launch((const unsigned char*)scratch, codes, powers, bias, C, part, M, N, m32, w16, steps, groups, p, epi, limit, stream);
+    };
     switch (p.form) {
-      case TILES: return tiles(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 3>{}, integral_constant<int, 1>{}, PAIR);
-      case TILES + 1: return tiles(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, PAIR);
-      case TILES + 2: return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 3>{}, integral_constant<int, 2>{}, PAIR);
-      default: return tiles(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, PAIR);
+      case TILES: return tiles(launch_tiles<256, 256, 3, 1, PAIR>);
+      case TILES + 1: return tiles(launch_tiles<256, 128, 2, 2, PAIR>);
+      case TILES + 2: return tiles(launch_tiles<128, 128, 3, 2, PAIR>);
+      default: return tiles(launch_tiles<64, 64, 4, 2, PAIR>);
     }
   };
   rc = epi == EPI_SWIGLU ? choose(std::true_type{}) : choose(std::false_type{});

@@ -4,6 +4,7 @@ import torch
 
 from minfer_amd.cli import main, parse_args
 from minfer_amd.kernels import ops
+from test_registers import _scratch_bytes
 from tiny import TINY_A
 
 
@@ -56,6 +57,18 @@ def test_a_limit_that_is_none(limit, monkeypatch):
     codes, powers = (torch.zeros(s, dtype=torch.uint8) for s in ops._mx4_pair_shapes(32, 64))
     with pytest.raises(ops.KernelError, match="limit"):
         ops.mx4_linear_swiglu(torch.zeros((3, 64)), codes, powers, torch.zeros((3, 32), dtype=torch.bfloat16), limit=limit)
+
+
+def test_streams_of_matrices_spill_nothing(tmp_path):
+    """As in the products of bfloat16 matrices: a reload would wait for the weights in flight."""
+    from minfer_amd.kernels import build
+    for name, kinds in (("gemm_mx4", ("few_kernel", "few_six_kernel", "rows_kernel")), ("moe_mx4", ("experts_up_kernel", "experts_down_kernel")),
+                        ("mx4", ("mx4_quantise_kernel", "mx4_dequantise_kernel"))):
+        if not build.is_current(name):
+            build.compile_library(name)
+        scratch = _scratch_bytes(build.lib_path(name), str(tmp_path))
+        assert all(any(k + "I" in n for n in scratch) for k in kinds)
+        assert not {n: b for n, b in scratch.items() if b and any(k + "I" in n for k in kinds)}
 
 
 def test_weights_option():

@@ -244,6 +244,42 @@ def test_operands_that_begin_anywhere(m):
         assert (around[:65] == 3).all() and (around[65 + m * n:] == 3).all()
 
 
+def guarded(shape, dtype, fill):
+    """A tensor of this shape in the middle of a larger one full of `fill`, and a check that nothing around it changed."""
+    n = torch.Size(shape).numel()
+    base = torch.full((n + 2 * 4096,), fill, dtype=dtype, device=DEV)
+    return base[4096:4096 + n].view(shape), lambda: bool((base[:4096] == fill).all() and (base[4096 + n:] == fill).all())
+
+
+@pytest.mark.parametrize("m", [1, 5, 8, 13, 16, 19, 37, 64, 75, 200, 513])
+@pytest.mark.parametrize("n,k", [(896, 896), (130, 1000), (37, 4097), (1003, 70)])
+def test_nothing_outside_is_written(m, n, k):
+    from minfer_amd.kernels import ops
+    w = normal((n, k), 3, std=0.05)
+    codes, codes_kept = guarded(ops.mx4_shapes(n, k)[0], torch.uint8, 0x5A)
+    powers, powers_kept = guarded(ops.mx4_shapes(n, k)[1], torch.uint8, 0x5A)
+    ops.mx4_quantise(w, codes, powers)
+    back, back_kept = guarded((n, k), BF16, -7.0)
+    ops.mx4_dequantise(codes, powers, back)
+    assert codes_kept() and powers_kept() and back_kept() and (back != -7.0).any()
+    x = normal((m, k), 4)
+    both = ops.mx4_pairs(codes, codes), ops.mx4_pairs(powers, powers)
+    for dtype, add in ((F32, False), (F32, True), (BF16, False)):
+        out, kept = guarded((m, n), dtype, -7.0)
+        ops.mx4_linear(x, codes, powers, None, out, accumulate=add)
+        assert kept() and (out != -7.0).float().mean() > 0.99
+    out, kept = guarded((m, n), BF16, -7.0)
+    ops.mx4_linear_swiglu(x, *both, out)
+    assert kept() and (out != -7.0).all()
+    if m <= 16:
+        down = quantised(normal((n, n), 5, std=0.05))
+        experts_ = [t[None].repeat(3, *[1] * t.dim()) for t in (*both, *down)]
+        chosen = torch.tensor([[i % 3, 2] for i in range(m)], dtype=torch.int32, device=DEV)
+        out, kept = guarded((m, n), BF16, -7.0)
+        ops.mx4_moe_sparse(x, *experts_, chosen, torch.ones((m, 2), device=DEV), out, n, act=1, accumulate=False)
+        assert kept() and (out != -7.0).float().mean() > 0.99
+
+
 def test_no_rows():
     from minfer_amd.kernels import ops
     codes, powers = quantised(normal((32, 64), 1))
