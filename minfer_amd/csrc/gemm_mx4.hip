@@ -216,9 +216,10 @@ __global__ __launch_bounds__(NW * 64) void few_six_kernel(const unsigned char* _
 }
 
 // ------------------------------------------------------------------ tiles
-// 1 KB from memory to LDS, lane after lane (its first byte in M0); the compiler does not know that it writes there, nor waits for it
-__device__ __forceinline__ void copy_kb(const void* base, unsigned off, unsigned lds_byte) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_byte) : "m0");
+// 1 KB from memory to LDS, lane after lane (its first byte, lds_byte + stage, in M0); the compiler does not know that it writes there, nor waits
+// for it
+__device__ __forceinline__ void copy_kb(const void* base, unsigned off, unsigned lds_byte, unsigned stage) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_byte), "s"(stage) : "m0", "scc");
 }
 // at most N of this wave's youngest copies are in flight, and all its LDS reads are back; then all waves meet
 template <int N>
@@ -329,19 +330,20 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   const unsigned lds0 = (unsigned)(uintptr_t)smem;
 
   // copies: piece q of this wave is piece 4 q + wid of the step (past the last: that one again, the same bytes to the same place)
-  const unsigned char *ga[TT::LA], *gw[TT::LW], *gp[TT::LP];
-  unsigned la[TT::LA], lw[TT::LW], lp[TT::LP], off_p[TT::LP];
-  const unsigned off = lane * 16;
+  // A step's bytes begin at `a0`, `w0` and a step's stride times its number, the same for all; a piece's place in it is the lane's.
+  const int a_first = bm * (BM / 32), w_first = bn * (BN / 16);
+  const unsigned char *a0 = a_codes + (size_t)a_first * steps * MX6_TILE, *w0 = w_codes + (size_t)w_first * steps * 1024, *gp[TT::LP];
+  unsigned la[TT::LA], lw[TT::LW], lp[TT::LP], off_a[TT::LA], off_w[TT::LW], off_p[TT::LP];
 #pragma unroll
   for (int q = 0; q < TT::LA; ++q) {
     const int piece = min(q * 4 + wid, TT::CA - 1), b = piece / 3, at = piece - b * 3;
-    ga[q] = a_codes + (size_t)min(bm * (BM / 32) + b, m32 - 1) * steps * MX6_TILE + at * 1024;
+    off_a[q] = (unsigned)min(b, m32 - 1 - a_first) * steps * MX6_TILE + at * 1024 + lane * 16;
     la[q] = lds0 + piece * 1024;
   }
 #pragma unroll
   for (int q = 0; q < TT::LW; ++q) {
     const int piece = min(q * 4 + wid, TT::CW - 1);
-    gw[q] = w_codes + (size_t)min(bn * (BN / 16) + piece, w16 - 1) * steps * 1024;
+    off_w[q] = (unsigned)min(piece, w16 - 1 - w_first) * steps * 1024 + lane * 16;
     lw[q] = lds0 + TT::A_ST + piece * 1024;
   }
 #pragma unroll
@@ -358,15 +360,19 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
     }
     lp[q] = lds0 + TT::STAGES * TT::STAGE + piece * 1024;
   }
-  auto copy = [&](int q, int t, int st) {                          // q: 0 .. L - 1
+  struct Bases { const unsigned char *a, *w; };
+  auto bases = [&](int t) {
     const int tc = min(t, last);
-    if (q < TT::LA) copy_kb(ga[q] + (size_t)tc * MX6_TILE, off, __builtin_amdgcn_readfirstlane(la[q] + st * TT::STAGE));
-    else copy_kb(gw[q - TT::LA] + (size_t)tc * 1024, off, __builtin_amdgcn_readfirstlane(lw[q - TT::LA] + st * TT::STAGE));
+    return Bases{a0 + (size_t)tc * MX6_TILE, w0 + (size_t)tc * 1024};
+  };
+  auto copy = [&](int q, const Bases& from, int st) {              // q: 0 .. L - 1
+    if (q < TT::LA) copy_kb(from.a, off_a[q], la[q], st * TT::STAGE);
+    else copy_kb(from.w, off_w[q - TT::LA], lw[q - TT::LA], st * TT::STAGE);
   };
   auto copy_powers = [&](int q, int group) {
     const int gc = min(group, g1 - 1);
     const bool a = q * 4 + wid < TT::NPA;
-    copy_kb(gp[q] + (size_t)gc * (a ? 512 : 256), off_p[q], __builtin_amdgcn_readfirstlane(lp[q] + (group & 1) * TT::POW));
+    copy_kb(gp[q] + (size_t)gc * (a ? 512 : 256), off_p[q], lp[q], (group & 1) * TT::POW);
   };
 
   // where this lane's operands lie in a stage
@@ -411,7 +417,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
 #pragma unroll
   for (int t = 0; t < STAGES; ++t)
 #pragma unroll
-    for (int q = 0; q < (t == STAGES - 1 ? EARLY : TT::L); ++q) copy(q, t0 + t, t);
+    for (int q = 0; q < (t == STAGES - 1 ? EARLY : TT::L); ++q) copy(q, bases(t0 + t), t);
   wait_and_meet<(STAGES - 2) * TT::L + EARLY>();
 #pragma unroll
   for (int z = 0; z < FIRST; ++z) read_first(z, 0, 0, true, g0);
@@ -419,6 +425,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   for (int j = 0; j < J; ++j) sw[j] = sw_next[j];
 
   int st = 0;
+  Bases late = bases(t0 + STAGES - 1);                             // of the step whose copies are set out in part
   auto step = [&](int t, int group, auto S) {
     constexpr int s = decltype(S)::value;
     const int next = st == STAGES - 1 ? 0 : st + 1;
@@ -430,11 +437,12 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
 #pragma unroll
       for (int z = q * (I / 2) / NM; z < (q + 1) * (I / 2) / NM; ++z) read_rows(I / 2 + z, st, s == 0, group);
 #pragma unroll
-      for (int z = q * (TT::L - EARLY) / NM; z < (q + 1) * (TT::L - EARLY) / NM; ++z) copy(EARLY + z, t + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
+      for (int z = q * (TT::L - EARLY) / NM; z < (q + 1) * (TT::L - EARLY) / NM; ++z) copy(EARLY + z, late, st == 0 ? STAGES - 1 : st - 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     // the second half's; behind the meeting this stage is free for the step after next but one, and the next step's operands are here.
     // In flight at the meeting: a step's copies, and at a group's second one the powers of the next group (set out behind the first).
+    late = bases(t + STAGES);
     constexpr int FLIGHT = (STAGES - 2) * TT::L + (s == 1 ? TT::LP : 0), COPIES = EARLY + (s == 0 ? TT::LP : 0);
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
         for (int z = b * FIRST / BEHIND; z < (b + 1) * FIRST / BEHIND; ++z) read_first(z, (s + 1) & 1, next, s == 3, group + 1);
 #pragma unroll
         for (int z = b * COPIES / BEHIND; z < (b + 1) * COPIES / BEHIND; ++z) {
-          if (z < EARLY) copy(z, t + STAGES, st);
+          if (z < EARLY) copy(z, late, st);
           else copy_powers(z - EARLY, group + 1);
         }
       }
@@ -620,7 +628,7 @@ static double result_bytes(int M, int N, int epi) { return (double)M * N * (epi 
 MF_API int mf_mx4_plan(int M, int N, int K, int epi, int whole, int n_cu, long long* out) {
   if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
   const long long w16 = (epi == EPI_SWIGLU ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30)) return (int)hipErrorInvalidValue;
+  if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30) || K > (1 << 24)) return (int)hipErrorInvalidValue;
   const Plan p = make_plan(M, (int)w16, (int)steps, whole, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
   out[0] = p.form;
   out[1] = p.splits;
