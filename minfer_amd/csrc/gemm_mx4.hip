@@ -51,13 +51,14 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
   const int step = group * 4 + (c >> 2), g = c & 3, r = row & 31;
   if (step < steps) {
     unsigned char* tile = codes + ((size_t)(row >> 5) * steps + step) * MX6_TILE;
-    *reinterpret_cast<uint4*>(tile + g * 512 + r * 16) = uint4{six[0], six[1], six[2], six[3]};
-    *reinterpret_cast<uint2*>(tile + 2048 + g * 256 + r * 8) = uint2{six[4], six[5]};
+    const int place = (r & 16) * 4 + g * 16 + (r & 15);
+    *reinterpret_cast<uint4*>(tile + place * 16) = uint4{six[0], six[1], six[2], six[3]};
+    *reinterpret_cast<uint2*>(tile + 2048 + place * 8) = uint2{six[4], six[5]};
   }
   unsigned four_powers = power << (8 * (c >> 2));
   four_powers |= __shfl_xor(four_powers, 4, MF_WAVE);
   four_powers |= __shfl_xor(four_powers, 8, MF_WAVE);
-  if (c < 4) powers[((size_t)(row >> 5) * groups + group) * 128 + g * 32 + r] = four_powers;
+  if (c < 4) powers[((size_t)(row >> 5) * groups + group) * 128 + (r & 16) * 4 + g * 16 + (r & 15)] = four_powers;
 }
 
 // ------------------------------------------------------------------ few rows
@@ -178,14 +179,13 @@ __global__ __launch_bounds__(NW * 64) void few_six_kernel(const unsigned char* _
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int r = (i & 1) * 16 + r16;
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         const unsigned char* tile = a_codes + ((size_t)(i >> 1) * steps + min(t0 + q, steps - 1)) * MX6_TILE;
-        x4[q][i] = *reinterpret_cast<const uint4*>(tile + g * 512 + r * 16);
-        x2[q][i] = *reinterpret_cast<const uint2*>(tile + 2048 + g * 256 + r * 8);
+        x4[q][i] = *reinterpret_cast<const uint4*>(tile + (i & 1) * 1024 + lane * 16);
+        x2[q][i] = *reinterpret_cast<const uint2*>(tile + 2048 + (i & 1) * 512 + lane * 8);
       }
-      xp[i] = a_powers[((size_t)(i >> 1) * groups + (t0 >> 2)) * 128 + g * 32 + r];
+      xp[i] = a_powers[((size_t)(i >> 1) * groups + (t0 >> 2)) * 128 + (i & 1) * 64 + lane];
     }
   };
   load(wid);
@@ -300,8 +300,8 @@ __device__ __forceinline__ void leave_rows(const unsigned char* __restrict__ own
 }
 
 // A workgroup of four waves (one a SIMD) takes a BM x BN tile of results, a wave a quarter of it in blocks of 16 x 16.
-// A step is 128 k: its codes are copied into one of the stages as they are stored (that is the order in which the operands' lanes read them,
-// 256 bytes to 16 lanes: no two lanes of a read meet in a bank), up to STAGES steps ahead; the powers of four steps likewise into one of two
+// A step is 128 k: its codes are copied into one of the stages as they are stored (that is the order in which the operands' lanes read them),
+// up to STAGES steps ahead; the powers of four steps likewise into one of two
 // places.  A step's products run in two halves, the upper half of the wave's rows and the lower: beside the first run the reads of the second's
 // rows, beside the second those of the next step's matrix and first rows, so that of the rows one step's operands are held and of the matrix
 // two.  The meeting in the second half says that the next step has landed and that nobody reads this one's stage any more.  Reads and copies are
@@ -309,6 +309,8 @@ __device__ __forceinline__ void leave_rows(const unsigned char* __restrict__ own
 // What bounds it: a prompt's products, the card's power and what is not beside products, a tile's first copies and its stores (4,096 rows, swiglu of
 // 37,888 x 3,584, 1.11 PFLOP: 346 us, 3.2 PFLOP/s; the same launch on zeros, which draw less, an eighth less; the products alone from registers
 // 6.9 PFLOP/s on values as they are here, 9.7 on zeros); hundreds of rows, the latency of a workgroup's own steps (300 rows of 2,048 x 2,048: 6.3 us).
+// Taken apart on 4,096 rows of 4,096 x 16,384 (256x256, the tile kernel alone, random values / zeros): 128 / 99 us; without copies 104 / 83, without
+// reads from LDS 123 / 99, products and meetings alone 101 / 74.
 // Why 16x16x128 and not 32x32x64: under the power limit the products alone run at 6.9 PFLOP/s instead of 5.9 (the whole launch above in 353 us
 // instead of 363, with the reads the same).
 template <int BM, int BN, int STAGES, int PER_CU, bool PAIR>
@@ -377,9 +379,9 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
 
   // where this lane's operands lie in a stage
   const int r16 = lane & 15, g = lane >> 4;
-  const unsigned a16 = wm * (I / 2) * MX6_TILE + g * 512 + r16 * 16, a8 = wm * (I / 2) * MX6_TILE + 2048 + g * 256 + r16 * 8;
+  const unsigned a16 = wm * (I / 2) * MX6_TILE + lane * 16, a8 = wm * (I / 2) * MX6_TILE + 2048 + lane * 8;
   const unsigned wb = TT::A_ST + wn * J * 1024 + lane * 16;
-  const unsigned pa = TT::STAGES * TT::STAGE + wm * (I / 2) * 512 + g * 128 + r16 * 4;
+  const unsigned pa = TT::STAGES * TT::STAGE + wm * (I / 2) * 512 + lane * 4;
   const unsigned pw = TT::STAGES * TT::STAGE + TT::PA + wn * J * 256 + lane * 4;
 
   floatx4 acc[I][J];
@@ -392,10 +394,10 @@ __global__ __launch_bounds__(256, PER_CU) void tile_kernel(const unsigned char* 
   // the operands of rows block i, of matrix block j (those of two steps in a row stand side by side), and their powers where a group begins
   auto read_rows = [&](int i, int st, bool begins, int group) {
     const int tile = i / 2, half = i % 2;
-    const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + tile * MX6_TILE + half * 256);
-    const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + tile * MX6_TILE + half * 128);
+    const uint4 x = *reinterpret_cast<const uint4*>(smem + st * TT::STAGE + a16 + tile * MX6_TILE + half * 1024);
+    const uint2 y = *reinterpret_cast<const uint2*>(smem + st * TT::STAGE + a8 + tile * MX6_TILE + half * 512);
     fa[i] = intx8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, 0, 0};
-    if (begins) sa[i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + tile * 512 + half * 64);
+    if (begins) sa[i] = *reinterpret_cast<const int*>(smem + (group & 1) * TT::POW + pa + tile * 512 + half * 256);
   };
   auto read_matrix = [&](int j, int side, int st, bool begins, int group) {
     fw[side][j] = mx4_operand(*reinterpret_cast<const uint4*>(smem + st * TT::STAGE + wb + j * 1024));
@@ -624,11 +626,12 @@ static Plan make_plan(int M, int w16, int steps, bool whole, bool pair, double o
 
 static double result_bytes(int M, int N, int epi) { return (double)M * N * (epi == EPI_SWIGLU || epi == EPI_BF16 ? 2 : 4); }
 
+// K: up to 2^23 (a piece's place in a tile stays below 2^31 bytes)
 // out: form, parts of K, bytes of scratch for the rows in E2M3, floats of scratch for the parts (64 bits each)
 MF_API int mf_mx4_plan(int M, int N, int K, int epi, int whole, int n_cu, long long* out) {
   if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
   const long long w16 = (epi == EPI_SWIGLU ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30) || K > (1 << 24)) return (int)hipErrorInvalidValue;
+  if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30) || K > (1 << 23)) return (int)hipErrorInvalidValue;
   const Plan p = make_plan(M, (int)w16, (int)steps, whole, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
   out[0] = p.form;
   out[1] = p.splits;

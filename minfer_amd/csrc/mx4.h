@@ -16,8 +16,9 @@
 // 32 g .. 32 g + 31 of the tile's 128, two a byte, the lower one in the low half: what lane 16 g + r of a wave feeds to
 // the 16x16x128 instruction, so a wave's load of a tile is one kilobyte without a gap.  Powers [ceil(rows / 16)][ceil(k / 512)][64][4 bytes]:
 // byte s of place 16 g + r is that of the block of tile 4 S + s: one load serves four steps.  Past the rows and past k: zeros.
-// Rows in 6 bits (scratch of a product), `[m][k]`: per 32 rows and 128 k three kilobytes: [4 g][32 r][16 bytes], the first 21 values and a third
-// of one, then [4 g][32 r][8 bytes]; powers [ceil(m / 32)][ceil(k / 512)][4 g][32 r][4 bytes].
+// Rows in 6 bits (scratch of a product), `[m][k]`: per 32 rows and 128 k three kilobytes: [2 halves][4 g][16 r][16 bytes], the first 21 values
+// and a third of one, then [2][4 g][16 r][8 bytes]; powers [ceil(m / 32)][ceil(k / 512)][2][4 g][16 r][4 bytes]: what the lanes 16 g + r of a
+// wave read lies without a gap, in LDS too (256 bytes to 16 lanes or 32: no two lanes of a read meet in a bank).
 #pragma once
 #include <type_traits>
 

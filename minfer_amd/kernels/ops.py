@@ -2274,7 +2274,7 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias:
                accumulate: bool = False) -> None:
     """out (+)= x' W'^T (+ bias): W' the matrix `[n][k]` that `codes`, `powers` hold in microscaled 4-bit numbers (`mx4_quantise`), x' the rows
     of `x` `[m][k]` (float32 or bfloat16) in microscaled 6-bit ones (E2M3: blocks of 32, the smallest power of two with which the largest magnitude is
-    at most 7.5, the nearest value, ties to even), which the product makes on its way.  Sums and `bias` are 32-bit; `out` `[m][n]` is float32, or
+    at most 7.5, the nearest value, ties to even), which the product makes on its way.  Sums and `bias` are 32-bit, k is at most 2^23; `out` `[m][n]` is float32, or
     bfloat16 where it is stored, and shares no memory with x.  A row of x with an infinity or a NaN gives NaN."""
     _need(x, "mx4_linear.x", _FLOATS)
     _need(out, "mx4_linear.out", _FLOATS)

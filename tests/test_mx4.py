@@ -51,6 +51,12 @@ def test_every_plan_covers_its_product(m, n, k):
         assert six == (0 if form == 0 else -(-m // 32) * (steps * 3 * 1024 + groups * 512))
 
 
+def test_sizes_that_no_product_takes():
+    for m, n, k in ((1, 16, (1 << 23) + 1), (1 << 30, 16, 1 << 20), (1, (1 << 30) + 1, 16)):
+        with pytest.raises(ops.KernelError, match="mx4_linear"):
+            ops._mx4_plan(m, n, k, ops.EPI_F32, True, 256)
+
+
 @pytest.mark.parametrize("limit", [-1.0, float("nan")])
 def test_a_limit_that_is_none(limit, monkeypatch):
     monkeypatch.setattr(ops, "_need", lambda *a: None)
