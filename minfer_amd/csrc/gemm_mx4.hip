@@ -627,11 +627,16 @@ static Plan make_plan(int M, int w16, int steps, bool whole, bool pair, double o
 static double result_bytes(int M, int N, int epi) { return (double)M * N * (epi == EPI_SWIGLU || epi == EPI_BF16 ? 2 : 4); }
 
 // K: up to 2^23 (a piece's place in a tile stays below 2^31 bytes)
+static bool sizes_fit(int M, int N, int K, int epi) {
+  if (M < 1 || N < 1 || K < 1 || K > (1 << 23)) return false;
+  const long long tiles = (epi == EPI_SWIGLU ? 2LL : 1LL) * ((N + 15LL) / 16), m32 = (M + 31LL) / 32, groups = (K + 511) / 512;
+  return tiles * 16 <= (1LL << 30) && m32 * 2 * groups <= (1LL << 30);
+}
+
 // out: form, parts of K, bytes of scratch for the rows in E2M3, floats of scratch for the parts (64 bits each)
 MF_API int mf_mx4_plan(int M, int N, int K, int epi, int whole, int n_cu, long long* out) {
-  if (M < 1 || N < 1 || K < 1 || n_cu < 1) return (int)hipErrorInvalidValue;
+  if (!sizes_fit(M, N, K, epi) || n_cu < 1) return (int)hipErrorInvalidValue;
   const long long w16 = (epi == EPI_SWIGLU ? 2LL : 1LL) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  if (w16 * 16 > (1LL << 30) || m32 * 2 * groups > (1LL << 30) || K > (1 << 23)) return (int)hipErrorInvalidValue;
   const Plan p = make_plan(M, (int)w16, (int)steps, whole, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
   out[0] = p.form;
   out[1] = p.splits;
@@ -644,8 +649,13 @@ template <int BM, int BN, int STAGES, int PER_CU, bool PAIR>
 static int launch_tiles(const unsigned char* six, const void* codes, const void* powers, const float* bias, void* C, float* part, int M, int N,
                         int m32, int w16, int steps, int groups, const Plan& p, int epi, float limit, hipStream_t stream) {
   using TT = Tile<BM, BN, STAGES>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<BM, BN, STAGES, PER_CU, PAIR>), hipFuncAttributeMaxDynamicSharedMemorySize, TT::LDS);
-  if (e != hipSuccess) return (int)e;
+  static bool configured = false;
+  if (!configured) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<BM, BN, STAGES, PER_CU, PAIR>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, TT::LDS);
+    if (e != hipSuccess) return (int)e;
+    configured = true;
+  }
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (w16 * 16 + BN - 1) / BN;
   tile_kernel<BM, BN, STAGES, PER_CU, PAIR><<<dim3(tiles_m * tiles_n, p.splits), 256, TT::LDS, stream>>>(
       six, six + (size_t)m32 * steps * MX6_TILE, (const unsigned char*)codes, (const unsigned char*)powers, bias, C, p.splits > 1 ? part : nullptr, M, N,
@@ -664,15 +674,18 @@ static int with_tiles(int epi, int w16, int n_cu, F run) {
 
 // C [M][N] (float32, added to where epi is EPI_ACC_F32, or bfloat16) from x [M][K] (bfloat16 or float32) and the stored [N][K]; EPI_SWIGLU: C is
 // [M][N] bfloat16 and the matrix holds N gate rows and N up rows, tile by tile in turn (limit above 0: the clamped gate with it).  scratch: as
-// `mf_mx4_plan` says, 16-byte aligned.
+// `mf_mx4_plan` says, 16-byte aligned; form, splits: its first two answers.
 MF_API int mf_mx4_linear(const void* x, int is_bf16, const void* codes, const void* powers, const float* bias, void* C, void* scratch, float* part,
-                         int M, int N, int K, int epi, float limit, int n_cu, hipStream_t stream) {
-  long long sizes[4];
+                         int M, int N, int K, int epi, float limit, int form, int splits, int n_cu, hipStream_t stream) {
+  if (!sizes_fit(M, N, K, epi) || n_cu < 1) return (int)hipErrorInvalidValue;
   const bool vec = (uintptr_t)x % 16 == 0 && K % (is_bf16 ? 8 : 4) == 0;
-  const int bad = mf_mx4_plan(M, N, K, epi, vec, n_cu, sizes);
-  if (bad) return bad;
   const int w16 = (epi == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16), m32 = (M + 31) / 32, steps = (K + 127) / 128, groups = (K + 511) / 512;
-  const Plan p = make_plan(M, w16, steps, vec, epi == EPI_SWIGLU, result_bytes(M, N, epi), n_cu);
+  // what the form takes: rows, and parts of K none of which is empty
+  if (form < FEW_RAW || form >= TILES + N_TILE_FORMS || (form == FEW_RAW && (M > 16 || !vec)) || (form == FEW_SIX && M > 64) || splits < 1 ||
+      splits > (form < TILES ? 1 : groups))
+    return (int)hipErrorInvalidValue;
+  const Plan p{form, splits, (groups + splits - 1) / splits};
+  if ((groups + p.groups - 1) / p.groups != splits) return (int)hipErrorInvalidValue;
   unsigned* a_powers = (unsigned*)((unsigned char*)scratch + (size_t)m32 * steps * MX6_TILE);
   if (p.form == FEW_RAW)
     return with_tiles(epi, w16, n_cu, [&](auto R0, auto PAIR) {

@@ -163,7 +163,7 @@ _PROTOTYPES = {
     },
     "gemm_mx4": {
         "mf_mx4_plan": [c_int, c_int, c_int, c_int, c_int, c_int, _P],
-        "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, c_int, _P],
+        "mf_mx4_linear": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, _P],
     },
     "moe_mx4": {
         "mf_mx4_moe": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
@@ -2263,11 +2263,12 @@ def _mx4_product(what: str, x: torch.Tensor, codes: torch.Tensor, powers: torch.
     if m == 0:
         return
     n_cu = cu_count()
-    _, _, six, parts = _mx4_plan(m, n, k, epi, _whole(x), n_cu)
+    form, splits, six, parts = _mx4_plan(m, n, k, epi, _whole(x), n_cu)
     # (of the call's own, not shared: calls on two streams, or two graphs, do not meet in them)
     scratch = torch.empty(six, dtype=torch.uint8, device=x.device) if six else None
     part = torch.empty(parts, dtype=torch.float32, device=x.device) if parts else None
-    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, limit, n_cu, _stream()), what)
+    _check(_fn("gemm_mx4", "mf_mx4_linear")(x, _is_bf16(x), codes, powers, bias, out, scratch, part, m, n, k, epi, limit, form, splits, n_cu, _stream()),
+           what)
 
 
 def mx4_linear(x: torch.Tensor, codes: torch.Tensor, powers: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
