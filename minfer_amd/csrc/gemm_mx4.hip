@@ -593,17 +593,20 @@ static double tile_cost(int f, int M, int w16, int steps, int splits, bool pair,
   return t.fixed + (t.each + (pair && splits == 1 ? t.gates : 0.)) * each + steps * std::max(t.step, t.step_each * each) + written;
 }
 
-// `whole`: rows of x whose 16-byte pieces begin at multiples of 16 bytes (as they come, `few_kernel` reads no others).
-// At most 16 rows, as they come or in E2M3 by a launch of their own in front: that launch costs some 2 us, quantising on the way as much as the
-// runs of a CU are many; what a run costs goes by how many rows share its lanes.  Microseconds, matrices from memory, as they come / in E2M3, by
-// U, the steps of a CU.  4 rows (any U): 4.1 / 6.2 (8,192 x 2,048, U 32), 12.5 / 12.9 (3,584 x 18,944, 148), 17.0 / 19.1 (37,888 x 3,584, 130).
-// 8 rows: 4.6 / 5.7 (3,584 x 3,584, 28), 9.0 / 8.6 (2,048 x 11,008, 86), 14.9 / 13.1 (148), 20.0 / 17.7 (130).  16 rows, from L2: 4.8 / 5.7
-// (2,048 x 2,048, 16), 6.3 / 6.3 (28), 11.3 / 7.7 (2,048 x 8,192, 64).
-static Plan make_plan(int M, int w16, int steps, bool whole, bool pair, double out_bytes, int n_cu) {
+// `whole`: 0 for rows of x whose 16-byte pieces do not begin at multiples of 16 bytes (as they come, `few_kernel` reads no others), 1 for bfloat16
+// ones that do, 2 for 32-bit ones.
+// At most 16 rows, as they come or in E2M3 by a launch of their own in front: that launch costs some 2 us; as they come a run of steps costs a CU
+// by its rows and their bytes (a lane reads 64 or 128 bytes of a row, a line or more to itself).  So it is the steps of a CU times the rows that
+// decides.  Microseconds, matrices from memory, as they come / in E2M3, by U, the steps of a CU.  bfloat16, 8 rows: 4.3 / 6.2 (3,584 x 3,584, U 28),
+// 21.0 / 22.3 (37,888 x 3,584, 140), 14.4 / 15.0 (3,584 x 18,944, 148; a matrix that lies in the memory-side cache 12.5 / 10.6); 12 rows: 5.5 / 6.1
+// (28), 6.3 / 6.0 (896 x 4,864, 38); 16 rows: 4.2 / 5.4 (2,048 x 2,048, 16), 6.2 / 6.1 (28).  32 bits, a row: 8.9 / 9.3 (2,048 x 11,008, 86), 16.0 / 15.0
+// (148); 4 rows: 5.7 / 6.0 (38), 13.0 / 9.4 (86); 8 rows: 4.4 / 5.4 (16), 8.0 / 6.1 (28); 16 rows: 5.7 / 4.9 (896 x 896, 7).
+static Plan make_plan(int M, int w16, int steps, int whole, bool pair, double out_bytes, int n_cu) {
   const int groups = (steps + 3) / 4;
   if (M <= 16) {
-    const long blocks = w16 > n_cu ? (w16 + 1) / 2 : w16, u = (blocks + n_cu - 1) / n_cu * steps;
-    return Plan{whole && (M <= 4 || u <= (M <= 8 ? 80 : 24)) ? FEW_RAW : FEW_SIX, 1, groups};
+    const long blocks = pair || w16 > n_cu ? (w16 + 1) / 2 : w16, u = (blocks + n_cu - 1) / n_cu * steps;
+    const long most = whole == 1 ? (M <= 8 ? 1120 : 448) : whole == 2 ? (M <= 8 ? 160 : 80) : -1;
+    return Plan{u * M <= most ? FEW_RAW : FEW_SIX, 1, groups};
   }
   // 17 to 64 rows: `few_six_kernel` by the steps of a CU's tiles (two and four tiles of rows: 6.5 + 0.054 us a step, 7.2 + 0.098; 69 products, 7 % rms off,
   // 17 % at most) against the tiles: 32 rows, 3,584 x 18,944 14.7 / 17.4 us; 64 rows 22.0 / 18.2, swiglu of 37,888 x 3,584 36.9 / 20.8.

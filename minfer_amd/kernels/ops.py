@@ -2243,16 +2243,17 @@ def mx4_dequantise(codes: torch.Tensor, powers: torch.Tensor, out: torch.Tensor)
     _check(_fn("mx4", "mf_mx4_dequantise")(codes, powers, out, _is_bf16(out), rows, k, _stream()), "mx4_dequantise")
 
 
-def _whole(x: torch.Tensor) -> bool:
-    """Whether every row of x begins at a multiple of 16 bytes."""
-    return not (x.data_ptr() % 16 or x.shape[1] % (8 if x.dtype == torch.bfloat16 else 4))
+def _whole(x: torch.Tensor) -> int:
+    """0 unless every row of x begins at a multiple of 16 bytes; then 1 for bfloat16 rows, 2 for float32 ones."""
+    half = x.dtype == torch.bfloat16
+    return 0 if x.data_ptr() % 16 or x.shape[1] % (8 if half else 4) else 1 if half else 2
 
 
 @functools.lru_cache(maxsize=4096)
-def _mx4_plan(m: int, n: int, k: int, epi: int, whole: bool, n_cu: int) -> Tuple[int, int, int, int]:
-    """(kernel, parts of K, bytes of scratch for the rows, floats of scratch for the parts); `whole`: x allows 16-byte loads."""
+def _mx4_plan(m: int, n: int, k: int, epi: int, whole: int, n_cu: int) -> Tuple[int, int, int, int]:
+    """(kernel, parts of K, bytes of scratch for the rows, floats of scratch for the parts); `whole`: `_whole(x)`."""
     out = (c_int64 * 4)()
-    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, epi, 1 if whole else 0, n_cu, out)
+    rc = _fn("gemm_mx4", "mf_mx4_plan")(m, n, k, epi, whole, n_cu, out)
     if rc != 0:
         raise KernelError(f"mx4_linear: error {rc} for m {m}, n {n}, k {k}")
     return tuple(out)

@@ -41,7 +41,7 @@ def test_host_tensors_are_refused():
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (896, 896), (3584, 18944), (4608, 3584), (152064, 3584), (100, 40000)])
 def test_every_plan_covers_its_product(m, n, k):
     """The parts of K of a plan cover it, none of them is empty, and the scratch is that of its kernels."""
-    for epi, whole in ((ops.EPI_F32, True), (ops.EPI_SWIGLU, True), (ops.EPI_BF16, False), (ops.EPI_SWIGLU, False)):
+    for epi, whole in ((ops.EPI_F32, 1), (ops.EPI_F32, 2), (ops.EPI_SWIGLU, 1), (ops.EPI_SWIGLU, 2), (ops.EPI_BF16, 0), (ops.EPI_SWIGLU, 0)):
         form, splits, six, parts = ops._mx4_plan(m, n, k, epi, whole, 256)
         groups, steps, w16 = -(-k // 512), -(-k // 128), -(-n // 16) * (2 if epi == ops.EPI_SWIGLU else 1)
         per = -(-groups // splits)
@@ -54,7 +54,7 @@ def test_every_plan_covers_its_product(m, n, k):
 def test_sizes_that_no_product_takes():
     for m, n, k in ((1, 16, (1 << 23) + 1), (1 << 30, 16, 1 << 20), (1, (1 << 30) + 1, 16)):
         with pytest.raises(ops.KernelError, match="mx4_linear"):
-            ops._mx4_plan(m, n, k, ops.EPI_F32, True, 256)
+            ops._mx4_plan(m, n, k, ops.EPI_F32, 1, 256)
 
 
 @pytest.mark.parametrize("limit", [-1.0, float("nan")])

@@ -137,7 +137,7 @@ TILED_GATES = [(2, False, 3484, 4102, 6683), (3, False, 772, 2662, 66), (3, True
 def planned(kernel, cut, m, n, k, epi):
     from minfer_amd.kernels import ops
     if ops.cu_count() == 256:
-        form, parts, _, _ = ops._mx4_plan(m, n, k, epi, True, 256)
+        form, parts, _, _ = ops._mx4_plan(m, n, k, epi, 1, 256)
         assert (form, parts > 1) == (kernel, cut)
 
 
