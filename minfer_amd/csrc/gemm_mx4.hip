@@ -65,7 +65,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, unsi
 // A workgroup owns R tiles of 16 matrix rows over the whole of K; its NW waves take the tiles' runs of G steps of 128 k in turn, so that at any
 // time they read neighbouring kilobytes, D runs of a wave in flight.  The waves' sums meet in LDS and are added in the waves' order.
 // What bounds it is the stream of the matrix; the rows come from L2 again for every workgroup.
-// (8 rows of 3,584 x 18,944 in E2M3, 36.1 MB of matrix: 8.2 us, 4.4 TB/s; 37,888 x 3,584, 72 MB: 13.1 us, 5.5 TB/s; a read without work reaches 6.3.)
+// (8 rows of 3,584 x 18,944 in E2M3, 36.1 MB of matrix: 8.1 us, 4.5 TB/s; as they come, 37,888 x 3,584, 72 MB: 13.4 us, 5.4 TB/s; a read without work
+// reaches 6.3.)
 
 // What the sums of 16 rows (from row m0 on) are joined to, of this thread's result: asked for in front of the stream, not behind it.
 template <int R, int NW>
@@ -307,7 +308,7 @@ __device__ __forceinline__ void leave_rows(const unsigned char* __restrict__ own
 // two.  The meeting in the second half says that the next step has landed and that nobody reads this one's stage any more.  Reads and copies are
 // set between the products one by one.
 // What bounds it: a prompt's products, the card's power and what is not beside products, a tile's first copies and its stores (4,096 rows, swiglu of
-// 37,888 x 3,584, 1.11 PFLOP: 346 us, 3.2 PFLOP/s; the same launch on zeros, which draw less, an eighth less; the products alone from registers
+// 37,888 x 3,584, 1.11 PFLOP: 345 us, 3.2 PFLOP/s; the same launch on zeros, which draw less, an eighth less; the products alone from registers
 // 6.9 PFLOP/s on values as they are here, 9.7 on zeros); hundreds of rows, the latency of a workgroup's own steps (300 rows of 2,048 x 2,048: 6.3 us).
 // Taken apart on 4,096 rows of 4,096 x 16,384 (256x256, the tile kernel alone, random values / zeros): 128 / 99 us; without copies 104 / 83, without
 // reads from LDS 123 / 99, products and meetings alone 101 / 74.
