@@ -20,13 +20,6 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // the gate of a product: silu, or with a limit above 0 the clamped form
 __device__ __forceinline__ float gate_mul(float g, float u, float limit) { return limit > 0.f ? clamped_gate(g, u, limit) : silu_mul(g, u); }
 
-// one value of a result that is not gated
-__device__ __forceinline__ void store_one(void* __restrict__ C, size_t at, float v, int epi) {
-  if (epi == EPI_BF16) ((bf16*)C)[at] = (bf16)v;
-  else if (epi == EPI_ACC_F32) ((float*)C)[at] += v;
-  else ((float*)C)[at] = v;
-}
-
 // ------------------------------------------------------------------ rows in E2M3
 // A wave takes four rows' 512 k, a lane a block of them, by way of LDS (`MxStage`; 4,096 rows of 3,584: 10.5 us, 3.9 TB/s; straight from the rows, 64
 // bytes a lane, 12.5.  37 rows of 2,500 that begin anywhere: 3.4; value by value in a lane 6.2).  Bound by memory: 2 or 4 bytes a value read, 25/32 written.
@@ -256,7 +249,8 @@ struct Tile {
 };
 
 // Results of more bytes than the L2s hold are marked: who reads them next finds them in no L2 anyway, and so they do not push the operands out.
-// (4,096 rows, swiglu of 37,888 x 3,584, 155 MB: 355 us, marked 329; 16,384 x 4,096 in 32 bits, 268 MB: 204, 189.)
+// (In bfloat16, 16,384 x 4,096 of K 4,096, 134 MB: 201 us, marked 187; 8,192 x 9,216 of K 2,048, 151 MB: 119, 114; swiglu of 4,096 rows, 155 MB: 329,
+// 326; of 38 MB, and in 32 bits, level.)
 __device__ __forceinline__ bool leaves_once(size_t bytes) { return bytes > (32u << 20); }
 
 // `rows` rows of COLS results that lie in LDS, `pitch` bytes to a row, to C [..][N] from row m_first and column n_first on: 32-bit ones (with a
@@ -569,18 +563,38 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
     }
     return v;
   };
+  // (four results in a store where C's rows allow it)
+  const bool whole = N % 4 == 0 && (uintptr_t)C % 16 == 0;
+  if (whole && c >= N) return;
+  const size_t to = (size_t)m * N + c;
+  float y[4];
   if (epi == EPI_SWIGLU) {
     const float4 g = sum((c >> 4) * 32 + (c & 15)), u = sum((c >> 4) * 32 + 16 + (c & 15));
-    const float y[4] = {gate_mul(g.x, u.x, limit), gate_mul(g.y, u.y, limit), gate_mul(g.z, u.z, limit), gate_mul(g.w, u.w, limit)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < N) ((bf16*)C)[(size_t)m * N + c + i] = (bf16)y[i];
+    y[0] = gate_mul(g.x, u.x, limit), y[1] = gate_mul(g.y, u.y, limit), y[2] = gate_mul(g.z, u.z, limit), y[3] = gate_mul(g.w, u.w, limit);
   } else {
     const float4 v = sum(c);
-    const float y[4] = {v.x, v.y, v.z, v.w};
+    y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (c + i < N) store_one(C, (size_t)m * N + c + i, bias ? y[i] + bias[c + i] : y[i], epi);
+      if (bias && c + i < N) y[i] += bias[c + i];
+  }
+  if (epi == EPI_SWIGLU || epi == EPI_BF16) {
+    if (whole) *reinterpret_cast<bf16x4*>((bf16*)C + to) = bf16x4{(bf16)y[0], (bf16)y[1], (bf16)y[2], (bf16)y[3]};
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < N) ((bf16*)C)[to + i] = (bf16)y[i];
+  } else {
+    float* at = (float*)C + to;
+    if (whole) {
+      float4 old = {0.f, 0.f, 0.f, 0.f};
+      if (epi == EPI_ACC_F32) old = *reinterpret_cast<const float4*>(at);
+      *reinterpret_cast<float4*>(at) = float4{old.x + y[0], old.y + y[1], old.z + y[2], old.w + y[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < N) at[i] = epi == EPI_ACC_F32 ? at[i] + y[i] : y[i];
+    }
   }
 }
 
